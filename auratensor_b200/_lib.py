@@ -23,7 +23,7 @@ AT_ERR_NCCL = -6
 AT_ERR_OOM = -7
 AT_ERR_TIMEOUT = -8
 
-GGML_F32, GGML_F16, GGML_Q4_0, GGML_Q8_0, GGML_Q6_K = 0, 1, 2, 8, 14
+GGML_F32, GGML_F16, GGML_Q4_0, GGML_Q8_0, GGML_Q6_K, GGML_BF16 = 0, 1, 2, 8, 14, 30
 # byte layouts of a model's tensors (include/auratensor.h AT_LAYOUT_*)
 LAYOUT_REFERENCE, LAYOUT_Q4_SPLIT_HALVES, LAYOUT_ATTN_OUT_IN, LAYOUT_LLAMA_CPP = 0, 1, 2, 3
 ORIENT_N, ORIENT_T = 0, 1
@@ -82,6 +82,23 @@ class SamplerConfigC(C.Structure):
                 ("repetition_penalty", C.c_float), ("seed", C.c_int64), ("history", C.c_void_p),
                 ("history_len", C.c_int32), ("reserved", C.c_int32)]
 
+
+class KvBlocksC(C.Structure):
+    """at_kvb: one layer of a block-quantized KV cache."""
+    _fields_ = [("dtype", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("block_tokens", C.c_int32),
+                ("n_blocks", C.c_int32), ("max_seqs", C.c_int32), ("max_blocks", C.c_int32), ("reserved", C.c_int32),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("k_tail", C.c_void_p), ("v_tail", C.c_void_p), ("k_tail_max", C.c_void_p), ("v_tail_max", C.c_void_p),
+                ("block_table", C.c_void_p), ("status", C.c_void_p)]
+
+
+class TokenBatchC(C.Structure):
+    """at_token_batch: runs of tokens, one per sequence."""
+    _fields_ = [("n_seqs", C.c_int32), ("n_tokens", C.c_int32), ("max_tokens", C.c_int32), ("reserved", C.c_int32),
+                ("max_end", C.c_int64), ("slots", C.c_void_p), ("starts", C.c_void_p), ("offsets", C.c_void_p)]
+
+
+KVB_BAD_SEQ, KVB_BAD_BLOCK = 1, 2
 
 _vp, _i, _i64, _sz, _f = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_float
 _PP = C.POINTER(C.c_void_p)
@@ -150,6 +167,11 @@ SIGNATURES = {
     "at_model_kv_append": [_vp, _i, _i64, _i64, _vp, _vp],
     "at_model_kv_offset": [_vp, _i64, _i64, _i64, _i64, C.POINTER(C.c_int64)],
     "at_sample": [_vp, _i, _vp, _i, _f, _i, _f, _f, _i64, C.POINTER(C.c_int)],
+    "at_kvb_append": [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64],
+    "at_kvb_read": [_vp, _vp, _vp, _i, _vp, _vp],
+    "at_kvb_attention": [_vp, _vp, _vp, _i, _i, _vp, _i64, _i64, _vp, _f, _i, _vp, _sz],
+    "at_kvb_attention_workspace": [_vp, _vp, _vp, _i, _i, C.POINTER(_sz)],
+    "at_logprobs": [_vp, _vp, _i, _i, _i, _i64, _vp, _i, _vp, _vp, _vp, _vp, _vp],
     "at_tp_unique_id": [_vp],
     "at_ctx_create_tp": [_i, _i, _i, _vp, _PP],
     "at_tp_shard_region": [_vp, _i, _i, C.c_char_p, _vp],

@@ -1,0 +1,333 @@
+// The block-quantized KV cache: K and V in 8 bits, one scale for each block of
+// tokens and KV head, blocks ("pages") found through a per-sequence table.
+//
+//   d = max|x| / 127 over the block's values so far (FP32 division; a d below
+//       2^-126 is held as 0, a NaN or infinity in the block makes d NaN, so
+//       that every read of the block gives NaN)
+//   q = round-half-even(x * (1 / d)), read back as q * d.
+//
+// A block fills token by token, and its scale grows with its maximum. The
+// original values of a sequence's last two blocks stay in a ring of 2 B rows
+// (the tail, with each row's max|x|), so when a new token raises the maximum
+// the block's older rows are quantized again from the originals: what a block
+// holds depends on its tokens alone, not on how appends cut them, and no
+// error builds up. Two blocks, so that the next append may also start
+// anywhere in the last block written or the one before it (a rejected draft
+// is overwritten).
+#include <cstdint>
+#include <string>
+
+#include "kvblock.cuh"
+
+namespace at {
+
+KvbDev kvb_dev(const at_ctx* ctx, const at_kvb* c, bool with_tail) {
+    AT_REQUIRE(ctx && c, AT_ERR_INVALID_ARG, "null argument");
+    AT_REQUIRE(c->dtype == AT_GGML_F32 || c->dtype == AT_GGML_F16 || c->dtype == AT_GGML_BF16, AT_ERR_UNSUPPORTED,
+               "cache type must be F32, F16 or BF16, got " + std::to_string(c->dtype));
+    AT_REQUIRE(c->head_dim == 64 || c->head_dim == 128, AT_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+    AT_REQUIRE(c->block_tokens == 16 || c->block_tokens == 32 || c->block_tokens == 64 || c->block_tokens == 128,
+               AT_ERR_INVALID_ARG, "block_tokens must be 16, 32, 64 or 128");
+    AT_REQUIRE(c->n_kv_heads > 0 && c->n_blocks > 0 && c->max_seqs > 0 && c->max_blocks > 0, AT_ERR_INVALID_ARG,
+               "cache dimensions must be positive");
+    AT_REQUIRE((int64_t)c->max_blocks * c->block_tokens <= INT32_MAX, AT_ERR_INVALID_ARG, "positions must fit 31 bits");
+    AT_REQUIRE(c->k && c->v && c->k_scale && c->v_scale && c->block_table, AT_ERR_INVALID_ARG, "null cache buffer");
+    AT_REQUIRE((((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0, AT_ERR_INVALID_ARG, "cache blocks must be 16-byte aligned");
+    if (with_tail) {
+        AT_REQUIRE(c->k_tail && c->v_tail && c->k_tail_max && c->v_tail_max, AT_ERR_STATE,
+                   "the cache has no tail buffers: it can only be read");
+        AT_REQUIRE((((uintptr_t)c->k_tail | (uintptr_t)c->v_tail) & 15) == 0, AT_ERR_INVALID_ARG,
+                   "tail buffers must be 16-byte aligned");
+    }
+    KvbDev d;
+    d.hkv = c->n_kv_heads;
+    d.hd = c->head_dim;
+    d.lb = c->block_tokens == 16 ? 4 : c->block_tokens == 32 ? 5 : c->block_tokens == 64 ? 6 : 7;
+    d.n_blocks = c->n_blocks;
+    d.max_seqs = c->max_seqs;
+    d.max_blocks = c->max_blocks;
+    d.k = c->k; d.v = c->v;
+    d.ks = c->k_scale; d.vs = c->v_scale;
+    d.kt = c->k_tail; d.vt = c->v_tail;
+    d.ktm = c->k_tail_max; d.vtm = c->v_tail_max;
+    d.table = c->block_table;
+    d.status = c->status;
+    return d;
+}
+
+KvbBatch kvb_batch(const at_kvb* c, const at_token_batch* b) {
+    AT_REQUIRE(b, AT_ERR_INVALID_ARG, "null batch");
+    AT_REQUIRE(b->n_seqs >= 0 && b->n_tokens >= 0 && b->max_tokens >= 0 && b->max_tokens <= b->n_tokens && b->max_end >= 0,
+               AT_ERR_INVALID_ARG, "bad batch sizes");
+    AT_REQUIRE(b->n_seqs == 0 || (b->slots && b->starts && b->offsets), AT_ERR_INVALID_ARG, "null batch buffer");
+    AT_REQUIRE(b->max_end <= (int64_t)c->max_blocks * c->block_tokens, AT_ERR_STATE,
+               "position " + std::to_string(b->max_end) + " is past the cache's " +
+                   std::to_string((int64_t)c->max_blocks * c->block_tokens) + " positions per sequence");
+    return KvbBatch{b->n_seqs, b->n_tokens, b->max_tokens, b->slots, b->starts, b->offsets};
+}
+
+namespace {
+
+constexpr int APPEND_THREADS = 256;
+constexpr uint32_t F32_INF = 0x7F800000u;
+
+// Eight consecutive elements as FP32; vec: p is 16-byte aligned.
+template <class T>
+__device__ __forceinline__ void load8(const T* __restrict__ p, bool vec, float* x) {
+    if (vec) {
+        alignas(16) T t[8];
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(t)[i] = reinterpret_cast<const uint4*>(p)[i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(t[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(p[i]);
+    }
+}
+template <class T>
+__device__ __forceinline__ void store8(T* __restrict__ p, const float* x) {
+    alignas(16) T t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = from_f32<T>(x[i]);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(t)[i];
+}
+
+// Bits of the largest |x| (as unsigned: finite < infinity < NaN).
+__device__ __forceinline__ uint32_t max_bits8(const float* x) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    return m;
+}
+
+__device__ __forceinline__ uint2 quant8(const float* x, float inv) {
+    uint32_t w[2] = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i >> 2] |= ((uint32_t)__float2int_rn(__fmul_rn(x[i], inv)) & 0xFFu) << (8 * (i & 3));
+    return make_uint2(w[0], w[1]);
+}
+
+template <class T>
+struct AppendSrc {
+    const T* x;
+    int64_t ts, hs;  // token and head strides, elements
+    bool vec;
+};
+
+// One CTA: one touched block of one sequence and KV head, of K or of V. The
+// block's new rows stay in registers (NCH chunks of 8 values per thread)
+// between the maximum and the quantization, so every value is read once.
+template <class T, int NCH>
+__global__ void __launch_bounds__(APPEND_THREADS) kvb_append_kernel(KvbDev c, KvbBatch b, AppendSrc<T> sk, AppendSrc<T> sv,
+                                                                    int max_touched) {
+    __shared__ uint32_t s_max[APPEND_THREADS / 32];
+    const int tid = threadIdx.x;
+    uint32_t w = blockIdx.x;
+    const bool is_v = w & 1;
+    w >>= 1;
+    const int h = w % c.hkv;
+    w /= c.hkv;
+    const int j = w % max_touched, s = w / max_touched;
+    const KvbSeq q = kvb_seq(c, b, s);
+    const int B = 1 << c.lb, hd = c.hd, cpr = hd >> 3;  // chunks per row
+    const int start = (int)q.start, end = start + q.n;
+    const int first = start >> c.lb, blk = first + j, base = blk << c.lb;
+    if (q.n == 0 || base >= end) return;
+    const int page = kvb_page(c, q.slot, blk);
+    if (page < 0) return;
+    const AppendSrc<T> src = is_v ? sv : sk;
+    const T* x0 = src.x + (int64_t)q.off * src.ts + (int64_t)h * src.hs;
+    const int lo = max(start, base), hi = min(end, base + B);
+    const size_t row0 = ((size_t)page * c.hkv + h) << c.lb;
+    int8_t* dst = (is_v ? c.v : c.k) + row0 * hd;
+    float* scale = (is_v ? c.vs : c.ks) + (size_t)page * c.hkv + h;
+    const size_t ring0 = ((size_t)q.slot * c.hkv + h) << (c.lb + 1);
+    T* tail = static_cast<T*>(is_v ? c.vt : c.kt) + ring0 * hd;
+    float* tail_max = (is_v ? c.vtm : c.ktm) + ring0;
+    const int last = (end - 1) >> c.lb;
+    const int ring_mask = 2 * B - 1;
+    // The rows of blocks last - 1 and last go to the ring. If this append
+    // begins inside a block and another block of the same parity is kept, the
+    // ring rows that the first block still reads are the ones that block
+    // overwrites: then the first block's CTA copies them, after its reads.
+    const bool open = start > (first << c.lb);
+    const int clash = (open && last >= first + 2) ? last - ((last - first) & 1) : -1;
+    const bool keep = blk >= last - 1 && blk != clash;
+
+    float x[NCH][8];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        const int ch = i * APPEND_THREADS + tid, r = ch / cpr, col = (ch - r * cpr) * 8;
+        const int p = base + r;
+        const bool live = p >= lo && p < hi && r < B;
+        uint32_t rm = 0;
+        if (live) {
+            load8<T>(x0 + (int64_t)(p - start) * src.ts + col, src.vec, x[i]);
+            rm = max_bits8(x[i]);
+        }
+        m = max(m, rm);
+        if (keep) {  // CTA-uniform; a row's chunks are cpr (8 or 16) neighbouring lanes
+            for (int o = cpr >> 1; o > 0; o >>= 1) rm = max(rm, __shfl_xor_sync(0xffffffffu, rm, o));
+            if (live) {
+                store8<T>(tail + (size_t)(p & ring_mask) * hd + col, x[i]);
+                if (col == 0) tail_max[p & ring_mask] = __uint_as_float(rm);
+            }
+        }
+    }
+    if (base + tid < lo) m = max(m, __float_as_uint(tail_max[(base + tid) & ring_mask]) & 0x7FFFFFFFu);
+    m = __reduce_max_sync(0xffffffffu, m);
+    if ((tid & 31) == 0) s_max[tid >> 5] = m;
+    const float held = *scale;  // the scale of the block's older rows
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < APPEND_THREADS / 32; ++i) m = max(m, s_max[i]);
+    float d = __fdiv_rn(__uint_as_float(m), 127.f), inv = 0.f;
+    if (m >= F32_INF) d = __uint_as_float(0x7FC00000u);
+    else if (d < 0x1p-126f) d = 0.f;
+    else inv = __fdiv_rn(1.f, d);
+    const bool poison = m >= F32_INF;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        const int ch = i * APPEND_THREADS + tid, r = ch / cpr, col = (ch - r * cpr) * 8;
+        if (base + r >= lo && base + r < hi && r < B)
+            *reinterpret_cast<uint2*>(dst + (size_t)r * hd + col) = poison ? make_uint2(0u, 0u) : quant8(x[i], inv);
+    }
+    if (__float_as_uint(held) != __float_as_uint(d)) {
+        for (int ch = tid; ch < (lo - base) * cpr; ch += APPEND_THREADS) {
+            const int r = ch / cpr, col = (ch - r * cpr) * 8;
+            float y[8];
+            load8<T>(tail + (size_t)((base + r) & ring_mask) * hd + col, true, y);
+            *reinterpret_cast<uint2*>(dst + (size_t)r * hd + col) = poison ? make_uint2(0u, 0u) : quant8(y, inv);
+        }
+        if (tid == 0) *scale = d;
+    }
+    if (j == 0 && clash >= 0) {
+        __syncthreads();  // every read of the ring rows is done
+        const int cb = clash << c.lb, n = min(end, cb + B) - cb;
+        for (int ch = tid; ch < B * cpr; ch += APPEND_THREADS) {  // whole warps: B * cpr is a multiple of 32
+            const int r = ch / cpr, col = (ch - r * cpr) * 8;
+            float y[8];
+            uint32_t rm = 0;
+            if (r < n) {
+                load8<T>(x0 + (int64_t)(cb + r - start) * src.ts + col, src.vec, y);
+                rm = max_bits8(y);
+                store8<T>(tail + (size_t)((cb + r) & ring_mask) * hd + col, y);
+            }
+            for (int o = cpr >> 1; o > 0; o >>= 1) rm = max(rm, __shfl_xor_sync(0xffffffffu, rm, o));
+            if (r < n && col == 0) tail_max[(cb + r) & ring_mask] = __uint_as_float(rm);
+        }
+    }
+}
+
+constexpr int READ_THREADS = 256;
+constexpr int READ_TOKENS = 32;  // positions per CTA
+
+// Four values per thread and step; a CTA reads READ_TOKENS positions of one
+// KV head, K or V, and writes them token-major.
+template <class T>
+__global__ void __launch_bounds__(READ_THREADS) kvb_read_kernel(KvbDev c, KvbBatch b, T* __restrict__ ok, T* __restrict__ ov,
+                                                                int chunks) {
+    uint32_t w = blockIdx.x;
+    const int h = w % c.hkv;
+    w /= c.hkv;
+    const int ch = w % chunks;
+    w /= chunks;
+    const bool is_v = ok ? (w & 1) : true;
+    const int s = (ok && ov) ? w >> 1 : w;
+    const KvbSeq q = kvb_seq(c, b, s);
+    const int i0 = ch * READ_TOKENS, n = min(READ_TOKENS, q.n - i0);
+    if (n <= 0) return;
+    const int8_t* src = is_v ? c.v : c.k;
+    const float* sc = is_v ? c.vs : c.ks;
+    T* out = is_v ? ov : ok;
+    const int per = c.hd >> 2;
+    for (int e = threadIdx.x; e < n * per; e += READ_THREADS) {
+        const int r = e / per, col = (e - r * per) * 4;
+        const int p = (int)q.start + i0 + r;
+        const int page = kvb_page(c, q.slot, p >> c.lb);
+        const size_t ph = (size_t)max(page, 0) * c.hkv + h;
+        const float d = page < 0 ? __uint_as_float(0x7FC00000u) : sc[ph];
+        const uint32_t x = *reinterpret_cast<const uint32_t*>(src + ((ph << c.lb) + (p & ((1 << c.lb) - 1))) * c.hd + col);
+        T* o = out + ((size_t)(q.off + i0 + r) * c.hkv + h) * c.hd + col;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = from_f32<T>(__fmul_rn((float)(int8_t)((x >> (8 * i)) & 0xFFu), d));
+    }
+}
+
+template <class T>
+void launch_append(const KvbDev& c, const KvbBatch& b, const AppendSrc<T>& k, const AppendSrc<T>& v, int64_t max_end,
+                   cudaStream_t s) {
+    const int B = 1 << c.lb;
+    const int touched = (b.max_tokens + B - 2) / B + 1;
+    const int64_t grid = (int64_t)b.n_seqs * touched * c.hkv * 2;
+    AT_REQUIRE(grid <= INT32_MAX, AT_ERR_INVALID_ARG, "the batch is too large for one append");
+    const int nch = B * c.hd / 8 / APPEND_THREADS;
+    switch (nch) {
+        case 8: kvb_append_kernel<T, 8><<<(int)grid, APPEND_THREADS, 0, s>>>(c, b, k, v, touched); break;
+        case 4: kvb_append_kernel<T, 4><<<(int)grid, APPEND_THREADS, 0, s>>>(c, b, k, v, touched); break;
+        case 2: kvb_append_kernel<T, 2><<<(int)grid, APPEND_THREADS, 0, s>>>(c, b, k, v, touched); break;
+        default: kvb_append_kernel<T, 1><<<(int)grid, APPEND_THREADS, 0, s>>>(c, b, k, v, touched); break;
+    }
+    AT_CUDA(cudaGetLastError());
+    (void)max_end;
+}
+
+template <class T>
+AppendSrc<T> append_src(const void* x, int64_t ts, int64_t hs) {
+    const int64_t per = 16 / (int64_t)sizeof(T);
+    AppendSrc<T> a{static_cast<const T*>(x), ts, hs, false};
+    a.vec = ((uintptr_t)x & 15) == 0 && ts % per == 0 && hs % per == 0;
+    return a;
+}
+
+}  // namespace
+
+}  // namespace at
+
+using namespace at;
+
+extern "C" {
+
+int at_kvb_append(at_ctx* ctx, const at_kvb* cache, const at_token_batch* batch, const void* k, int64_t k_token_stride,
+                  int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride) {
+    return guard([&] {
+        const KvbDev c = kvb_dev(ctx, cache, true);
+        const KvbBatch b = kvb_batch(cache, batch);
+        if (b.n_seqs == 0 || b.max_tokens == 0) return;
+        AT_REQUIRE(k && v, AT_ERR_INVALID_ARG, "null K or V");
+        const uintptr_t e = kvb_elem_bytes(cache->dtype);
+        AT_REQUIRE((((uintptr_t)k | (uintptr_t)v) & (e - 1)) == 0, AT_ERR_INVALID_ARG, "K and V must be aligned to their elements");
+        AT_CUDA(cudaSetDevice(ctx->device));
+        kvb_dispatch(cache->dtype, [&](auto t) {
+            using T = decltype(t);
+            launch_append<T>(c, b, append_src<T>(k, k_token_stride, k_head_stride),
+                             append_src<T>(v, v_token_stride, v_head_stride), batch->max_end, ctx->stream);
+        });
+    });
+}
+
+int at_kvb_read(at_ctx* ctx, const at_kvb* cache, const at_token_batch* batch, int out_type, void* k_out, void* v_out) {
+    return guard([&] {
+        const KvbDev c = kvb_dev(ctx, cache, false);
+        const KvbBatch b = kvb_batch(cache, batch);
+        AT_REQUIRE(out_type == AT_GGML_F32 || out_type == AT_GGML_F16 || out_type == AT_GGML_BF16, AT_ERR_UNSUPPORTED,
+                   "output type must be F32, F16 or BF16");
+        if (b.n_seqs == 0 || b.max_tokens == 0) return;
+        AT_REQUIRE(k_out || v_out, AT_ERR_INVALID_ARG, "null outputs");
+        AT_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, AT_ERR_INVALID_ARG, "outputs must be 16-byte aligned");
+        const int chunks = (b.max_tokens + READ_TOKENS - 1) / READ_TOKENS;
+        const int64_t grid = (int64_t)b.n_seqs * (k_out && v_out ? 2 : 1) * chunks * c.hkv;
+        AT_REQUIRE(grid <= INT32_MAX, AT_ERR_INVALID_ARG, "the batch is too large for one read");
+        AT_CUDA(cudaSetDevice(ctx->device));
+        kvb_dispatch(out_type, [&](auto t) {
+            using T = decltype(t);
+            kvb_read_kernel<T><<<(int)grid, READ_THREADS, 0, ctx->stream>>>(c, b, static_cast<T*>(k_out), static_cast<T*>(v_out), chunks);
+        });
+        AT_CUDA(cudaGetLastError());
+    });
+}
+
+}  // extern "C"

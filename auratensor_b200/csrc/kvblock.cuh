@@ -1,0 +1,105 @@
+// Shared by the kernels of the block-quantized KV cache (kvblock.cu,
+// kvblock_attn.cu): the cache and batch descriptors on the device, and the
+// checks that keep a bad descriptor from turning into a bad address.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "at_internal.h"
+#include "dev_common.cuh"
+
+namespace at {
+
+// Bits of the cache's status word (at_kvb.status).
+constexpr int KVB_BAD_SEQ = 1;    // a slot, start or offset outside its range: the sequence was skipped
+constexpr int KVB_BAD_BLOCK = 2;  // a block-table entry outside the pool: reads give NaN, writes are dropped
+
+struct KvbDev {
+    int hkv, hd, lb;  // lb: log2(block_tokens)
+    int n_blocks, max_seqs, max_blocks;
+    int8_t *k, *v;
+    float *ks, *vs;
+    void *kt, *vt;
+    float *ktm, *vtm;
+    const int32_t* table;
+    int32_t* status;
+};
+
+struct KvbBatch {
+    int n_seqs, n_tokens, max_tokens;
+    const int32_t* slots;
+    const int64_t* starts;
+    const int32_t* offsets;
+};
+
+// Host checks (kvblock.cu); fail() with the framework's status classes.
+KvbDev kvb_dev(const at_ctx* ctx, const at_kvb* c, bool with_tail);
+KvbBatch kvb_batch(const at_kvb* c, const at_token_batch* b);
+
+struct KvbSeq {
+    int slot, n, off;
+    int64_t start;
+};
+
+__device__ __forceinline__ void kvb_flag(int32_t* status, int bit) {
+    if (status) atomicOr(status, bit);
+}
+
+// Sequence s of the batch; n = 0 (and the status bit) when it is out of range.
+__device__ __forceinline__ KvbSeq kvb_seq(const KvbDev& c, const KvbBatch& b, int s) {
+    KvbSeq q;
+    q.slot = b.slots[s];
+    q.start = b.starts[s];
+    q.off = b.offsets[s];
+    q.n = b.offsets[s + 1] - q.off;
+    const int64_t room = (int64_t)c.max_blocks << c.lb;
+    if (q.n < 0 || q.n > b.max_tokens || q.off < 0 || q.off > b.n_tokens - q.n || (unsigned)q.slot >= (unsigned)c.max_seqs ||
+        q.start < 0 || q.start > room - q.n) {
+        kvb_flag(c.status, KVB_BAD_SEQ);
+        q.n = 0;
+    }
+    return q;
+}
+
+// Page of a sequence's block, or -1 (and the status bit).
+__device__ __forceinline__ int kvb_page(const KvbDev& c, int slot, int blk) {
+    const int p = c.table[(size_t)slot * c.max_blocks + blk];
+    if ((unsigned)p < (unsigned)c.n_blocks) return p;
+    kvb_flag(c.status, KVB_BAD_BLOCK);
+    return -1;
+}
+
+template <class T>
+__device__ __forceinline__ float to_f32(T x);
+template <>
+__device__ __forceinline__ float to_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+template <class T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// Calls f with a value of the C++ type of a dtype code.
+template <class F>
+inline void kvb_dispatch(int dtype, F&& f) {
+    switch (dtype) {
+        case AT_GGML_F32: f(float{}); return;
+        case AT_GGML_F16: f(__half{}); return;
+        case AT_GGML_BF16: f(__nv_bfloat16{}); return;
+        default: fail(AT_ERR_UNSUPPORTED, "element type must be F32, F16 or BF16, got " + std::to_string(dtype));
+    }
+}
+inline int kvb_elem_bytes(int dtype) { return dtype == AT_GGML_F32 ? 4 : 2; }
+
+}  // namespace at

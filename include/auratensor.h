@@ -41,6 +41,7 @@ extern "C" {
 #define AT_GGML_Q4_0  2
 #define AT_GGML_Q8_0  8
 #define AT_GGML_Q6_K 14
+#define AT_GGML_BF16 30  /* activations of the block-quantized cache and of at_logprobs; not a weight type here */
 
 /* Byte layouts of a model's tensors. 0 is the reference's: Q4_0 nibbles
  * interleaved (element 2k = low nibble of byte k, quant/Q4_0.java:21-22) and
@@ -349,6 +350,95 @@ int at_model_kv_offset(const at_model* m, int64_t layer, int64_t kv_head, int64_
 /* ---- sampler: Sampler.sample (inference/Sampler.java:37-121), host -------- */
 int at_sample(float* logits, int vocab, const int* history, int n_history, float temperature,
               int top_k, float top_p, float repetition_penalty, int64_t seed, int* out_token);
+
+/* ---- block-quantized KV cache: paged, 8 bits, one scale per block and head --
+ * New (the reference keeps K and V in FP32, inference/KVCache.java:56-61). One
+ * at_kvb describes one layer's cache in device memory that the caller owns;
+ * layers share block_table and differ in their buffers. Position p of a
+ * sequence (its slot: a row of block_table) lives in row p % block_tokens of
+ * page block_table[slot][p / block_tokens]. Per page and KV head one FP32
+ * scale d covers block_tokens x head_dim values:
+ *   d = max|x| / 127 (0 below 2^-126; NaN when a value is NaN or infinite, so
+ *   every read of that block gives NaN), q = round-half-even(x * (1 / d)),
+ *   read back as q * d.
+ * The tail rings hold the original values of the last two blocks of each slot
+ * (row p % (2 block_tokens)) with each row's max|x|: when a new token raises
+ * an open block's maximum, its older rows are quantized again from them, so a
+ * block's contents depend on its tokens alone, not on how appends cut them.
+ * Pages that are full are never written again and may be shared by slots. */
+typedef struct at_kvb {
+    int32_t dtype;                 /* type of appended K/V and of the tail: AT_GGML_F32, _F16, _BF16 */
+    int32_t n_kv_heads;
+    int32_t head_dim;              /* 64 or 128 */
+    int32_t block_tokens;          /* 16, 32, 64 or 128 */
+    int32_t n_blocks;              /* pages in the pool */
+    int32_t max_seqs;              /* slots */
+    int32_t max_blocks;            /* pages per slot at most */
+    int32_t reserved;
+    int8_t* k;                     /* [n_blocks][n_kv_heads][block_tokens][head_dim] */
+    int8_t* v;
+    float* k_scale;                /* [n_blocks][n_kv_heads] */
+    float* v_scale;
+    void* k_tail;                  /* [max_seqs][n_kv_heads][2 block_tokens][head_dim], dtype; all four */
+    void* v_tail;                  /* tail buffers may be NULL for a cache that is only read */
+    float* k_tail_max;             /* [max_seqs][n_kv_heads][2 block_tokens] */
+    float* v_tail_max;
+    const int32_t* block_table;    /* [max_seqs][max_blocks] */
+    int32_t* status;               /* one word or NULL: AT_KVB_BAD_* bits are set when a kernel meets them */
+} at_kvb;
+#define AT_KVB_BAD_SEQ   1         /* slot, start or offset out of range: that sequence was skipped */
+#define AT_KVB_BAD_BLOCK 2         /* block_table entry outside the pool: writes dropped, reads NaN */
+/* Runs of consecutive tokens, one per sequence, packed one after the other:
+ * sequence s has slot slots[s] and the tokens offsets[s] .. offsets[s+1] of the
+ * packed arrays, at positions starts[s], starts[s] + 1, ... The arrays are on
+ * the device (a captured graph can advance them); the maxima are the host's
+ * and bound the launches. A slot appears once at most. */
+typedef struct at_token_batch {
+    int32_t n_seqs;
+    int32_t n_tokens;              /* all runs together */
+    int32_t max_tokens;            /* of the longest run */
+    int32_t reserved;
+    int64_t max_end;               /* highest position + 1; past the cache's positions: AT_ERR_STATE */
+    const int32_t* slots;          /* [n_seqs] */
+    const int64_t* starts;         /* [n_seqs] */
+    const int32_t* offsets;        /* [n_seqs + 1] */
+} at_token_batch;
+/* Writes the batch's K and V ([n_tokens][n_kv_heads][head_dim] of the cache's
+ * dtype, head_dim contiguous, strides in elements; the KVCache.append of this
+ * cache, inference/KVCache.java:79-95). A run may start anywhere from the
+ * first position of the block before the slot's last written one: what lies
+ * after it is overwritten. Runs on the context's stream. */
+int at_kvb_append(at_ctx* ctx, const at_kvb* cache, const at_token_batch* batch, const void* k, int64_t k_token_stride,
+                  int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride);
+/* Reads the batch's positions back as values, [n_tokens][n_kv_heads][head_dim]
+ * of out_type; k_out or v_out may be NULL. */
+int at_kvb_read(at_ctx* ctx, const at_kvb* cache, const at_token_batch* batch, int out_type, void* k_out, void* v_out);
+/* Causal attention of the batch's query tokens over what the cache holds of
+ * their sequences (LlamaModel.attention, inference/LlamaModel.java:255-297):
+ * the query at position p sees the keys j <= p, with window > 0 only
+ * j > p - window. q: [n_tokens][n_heads][head_dim] of dtype (strides in
+ * elements), out the same shape, contiguous; query head h reads KV head
+ * h n_kv_heads / n_heads. The tokens themselves are appended first. Decode
+ * steps and prompts are the same call. Statistics and sums are FP32.
+ * workspace: device memory of at_kvb_attention_workspace bytes (may be 0),
+ * free for other use when the call's work on the stream is done. */
+int at_kvb_attention(at_ctx* ctx, const at_kvb* cache, const at_token_batch* batch, int dtype, int n_heads, const void* q,
+                     int64_t q_token_stride, int64_t q_head_stride, void* out, float scale, int window, void* workspace,
+                     size_t workspace_bytes);
+int at_kvb_attention_workspace(at_ctx* ctx, const at_kvb* cache, const at_token_batch* batch, int n_heads, int window,
+                               size_t* bytes);
+
+/* ---- log probabilities ------------------------------------------------------
+ * Per row of logits [rows][vocab] (dtype F32, F16 or BF16, row_stride
+ * elements apart): logsumexp, the entropy of softmax(logits) in nats, the log
+ * probability of tokens[row] (tokens and logprob NULL together; an id outside
+ * [0, vocab): NaN), and the n_top <= 32 most likely ids in descending order
+ * with their log probabilities (equal logits: lower id first). -inf logits
+ * have probability 0. A row of -inf only: logsumexp -inf, log probabilities
+ * -inf, entropy 0. A row with NaN or +inf: NaN (ids as ordered, NaN first).
+ * The logits are not changed. New (the reference returns sampled ids only). */
+int at_logprobs(at_ctx* ctx, const void* logits, int dtype, int rows, int vocab, int64_t row_stride, const int32_t* tokens,
+                int n_top, float* logprob, float* logsumexp, float* entropy, int32_t* top_ids, float* top_logprobs);
 
 /* ---- tensor parallelism over NCCL (new: the reference is single-process) --- */
 /* 128-byte ncclUniqueId for rank 0 to broadcast to the other ranks. */
