@@ -6,6 +6,7 @@
 // with m the running maximum; statistics and sums in FP32. A hidden key is
 // left out by its index, so what its bytes or scale hold never matters; a
 // visible key of a poisoned block (scale NaN) makes the row NaN.
+#include <algorithm>
 #include <cstdint>
 #include <string>
 
@@ -15,6 +16,435 @@ namespace at {
 
 namespace {
 
+// ---------------------------------------------------------------------------
+// Few query rows per KV head (decode steps, drafted tokens)
+// ---------------------------------------------------------------------------
+// Rows r = token * G + query head of one (sequence, KV head) form the N side
+// (8 per tile, NT tiles) of mma.sync m16n8k16 (f16 operands, FP32 sums); keys
+// are the M side of S^T = K Q^T, head dimensions the M side of O^T = V^T P^T.
+// Both A operands are built in registers from the int8 bytes as they come
+// from memory, exact in f16 (|q| <= 127), so K and V cross shared memory
+// nowhere: a warp's unit is 64 keys, 16-byte loads straight into the lanes
+// that multiply them. Which key or dimension a lane's bytes are is free, as
+// long as both operands agree, and is chosen so that
+//   K: lane (g, t) holds 16 bytes of key rows 16 (g / 2) + 4 j + (g & 1), + 2;
+//   V: lane (g, t) holds HD / 8 bytes of keys 16 t + 4 j .. + 3;
+//   the S^T accumulators, packed to f16 pairs and transposed by movmatrix,
+//   are the P^T operand.
+// tcgen05 would want the converted tiles in shared memory and 128 rows; here
+// there are 8 or 16 and the time goes to the K and V bytes.
+// FP32 queries are split into two f16 parts (22 bits), and so are the weights;
+// F16/BF16 queries are exact in one (each row is scaled by a power of two
+// into f16's range) and their weights are rounded once to 11 bits. Weights
+// carry d_v relative to a running reference D (at least every d_v so far), so
+// they stay in f16's range whatever the values' scale; O is kept in units of D.
+constexpr int ST_WARPS = 4;
+constexpr int ST_THREADS = 32 * ST_WARPS;
+constexpr int ST_UNIT = 64;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {  // a in the low half
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_h2(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+// Two biased bytes (q + 128) of w, selected with 0x64 above each: 1024 + q + 128
+// as f16 pairs; minus 1152 is q, exactly.
+template <int SEL>
+__device__ __forceinline__ uint32_t bytes_h2(uint32_t w) {
+    const uint32_t m = __byte_perm(w, 0x64646464u, SEL);
+    const uint32_t c = 0x64806480u;
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&m), *reinterpret_cast<const __half2*>(&c));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <int N>
+struct Bytes;
+template <>
+struct Bytes<16> { uint32_t w[4]; };
+template <>
+struct Bytes<8> { uint32_t w[2]; };
+__device__ __forceinline__ void ld_bytes(Bytes<16>& b, const int8_t* p) {
+    const uint4 v = ld_stream_u4(p);
+    b.w[0] = v.x; b.w[1] = v.y; b.w[2] = v.z; b.w[3] = v.w;
+}
+__device__ __forceinline__ void ld_bytes(Bytes<8>& b, const int8_t* p) {
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(b.w[0]), "=r"(b.w[1]) : "l"(p));
+}
+
+// Power of two that brings a row whose largest |x| is `top` to [512, 1024).
+__device__ __forceinline__ float row_scale(float top) {
+    const int e = (int)(__float_as_uint(top) >> 23) - 127;  // -127: zero or subnormal
+    return __uint_as_float((uint32_t)(127 + min(9 - e, 126)) << 23);
+}
+
+struct StepParams {
+    KvbDev c;
+    KvbBatch b;
+    const void* q;
+    int64_t q_ts, q_hs;
+    void* out;
+    int H, G, groups, splits, window, max_rows;  // groups: row groups of 8 NT; sequences above max_rows rows are skipped
+    float scale;
+    float* part_o;   // [item][split][8 NT][HD]
+    float2* part_ml; // [item][split][8 NT]
+};
+
+template <class T, int HD, int NT>
+__global__ void __launch_bounds__(ST_THREADS) kvb_attn_step_kernel(const StepParams p) {
+    constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
+    constexpr int KS = HD / 16;    // k-steps of K Q^T
+    constexpr int KC = HD / 64;    // 16-byte chunks of a key row per lane
+    constexpr int MT = HD / 16;    // M tiles of V^T P^T
+    constexpr int VB = HD / 8;     // bytes of a value row per lane
+    constexpr int ROWS = 8 * NT;
+    const KvbDev& c = p.c;
+    __shared__ float s_ml[ST_WARPS][ROWS][2];
+    __shared__ float s_o[ST_WARPS][ROWS][HD];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int item = blockIdx.x / p.splits, split = blockIdx.x - item * p.splits;
+    const int rg = item % p.groups, kvh = (item / p.groups) % c.hkv, s = item / p.groups / c.hkv;
+    const KvbSeq sq = kvb_seq(c, p.b, s);
+    const int R = sq.n * p.G, r0 = rg * ROWS;
+    if (r0 >= R || R > p.max_rows) return;
+    const int start = (int)sq.start;
+    const int first_pos = start + r0 / p.G, last_pos = start + (min(R, r0 + ROWS) - 1) / p.G;
+    const int lo = p.window > 0 ? max(0, first_pos - p.window + 1) : 0, hi = last_pos + 1;
+    const int u_lo = lo / ST_UNIT, nu = (hi - 1) / ST_UNIT + 1 - u_lo;
+    const int u0 = u_lo + (int)((int64_t)nu * split / p.splits), u1 = u_lo + (int)((int64_t)nu * (split + 1) / p.splits);
+
+    // queries: row g of each tile, 4 dims per k-step
+    uint32_t qf[NT][TERMS][KS][2];
+    float qs[NT][2];  // score factors of rows 2 t, 2 t + 1 (log2 units)
+    int qp[NT][2];    // their positions (padding rows: -1, they see nothing)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = r0 + 8 * nt + g;
+        float x[KC][16];
+        float top = 0.f;
+#pragma unroll
+        for (int cc = 0; cc < KC; ++cc)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                x[cc][i] = r < R ? to_f32<T>(static_cast<const T*>(p.q)[(int64_t)(sq.off + r / p.G) * p.q_ts +
+                                                                      (int64_t)(kvh * p.G + r % p.G) * p.q_hs + 64 * cc + 16 * t + i])
+                                 : 0.f;
+                top = fmaxf(top, fabsf(x[cc][i]));
+            }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float rs = row_scale(top);
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const float a0 = x[kk >> 2][4 * (kk & 3) + 2 * b] * rs, a1 = x[kk >> 2][4 * (kk & 3) + 2 * b + 1] * rs;
+                const uint32_t hi2 = pack_h2(a0, a1);
+                qf[nt][0][kk][b] = hi2;
+                if constexpr (TERMS == 2) {
+                    const float2 h = unpack_h2(hi2);
+                    qf[nt][1][kk][b] = pack_h2(a0 - h.x, a1 - h.y);
+                }
+            }
+        const float f = p.scale * 1.44269504088896341f / rs;  // exact division: rs is a power of two
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            qs[nt][e] = __shfl_sync(0xffffffffu, f, (2 * t + e) * 4);
+            const int rr = r0 + 8 * nt + 2 * t + e;
+            qp[nt][e] = rr < R ? start + rr / p.G : -1;
+        }
+    }
+
+    float o[NT][MT][4];
+    float m[NT][2], l[NT][2], D = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+        m[nt][0] = m[nt][1] = -INFINITY;
+        l[nt][0] = l[nt][1] = 0.f;
+    }
+
+    // page of this lane's sub-block t of a unit (-2: past the last key, -1: outside the pool)
+    auto lookup = [&](int u) { return (u < u1 && u * ST_UNIT + 16 * t < hi) ? kvb_page(c, sq.slot, (u * ST_UNIT + 16 * t) >> c.lb) : -2; };
+    const int bmask = (1 << c.lb) - 1;
+    auto load_k = [&](Bytes<16> (&kr)[4][2][KC], int u, int pk) {  // pk: page of sub-block g / 2
+        const int8_t* base = c.k + ((((size_t)max(pk, 0) * c.hkv + kvh) << c.lb) + ((u * ST_UNIT + 16 * (g >> 1)) & bmask)) * HD + 16 * t;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int cc = 0; cc < KC; ++cc) ld_bytes(kr[j][e][cc], base + (4 * j + (g & 1) + 2 * e) * HD + 64 * cc);
+    };
+    auto load_d = [&](int pk, float* dk, float* dv) {
+        const size_t i = (size_t)max(pk, 0) * c.hkv + kvh;
+        *dk = pk == -1 ? __uint_as_float(0x7FC00000u) : pk < 0 ? 0.f : c.ks[i];
+        *dv = pk == -1 ? __uint_as_float(0x7FC00000u) : pk < 0 ? 0.f : c.vs[i];
+    };
+
+    int u = u0 + warp;
+    int pv = lookup(u), pv_next = lookup(u + ST_WARPS);
+    Bytes<16> kr[4][2][KC];
+    float dk, dv;
+    {
+        const int pk = __shfl_sync(0xffffffffu, pv, g >> 1);
+        load_k(kr, u, pk);
+        load_d(pk, &dk, &dv);
+    }
+    for (; u < u1; u += ST_WARPS) {
+        // the values' bytes are asked for before the keys are multiplied
+        Bytes<VB> vr[4][4];
+        {
+            const int8_t* base = c.v + ((((size_t)max(pv, 0) * c.hkv + kvh) << c.lb) + ((u * ST_UNIT + 16 * t) & bmask)) * HD + VB * g;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ld_bytes(vr[j][e], base + (4 * j + e) * HD);
+        }
+        float sc[4][NT][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) sc[j][nt][0] = sc[j][nt][1] = sc[j][nt][2] = sc[j][nt][3] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk) {
+                const uint32_t w0 = kr[j][0][kk >> 2].w[kk & 3] ^ 0x80808080u, w1 = kr[j][1][kk >> 2].w[kk & 3] ^ 0x80808080u;
+                const uint32_t a0 = bytes_h2<0x4140>(w0), a1 = bytes_h2<0x4140>(w1), a2 = bytes_h2<0x4342>(w0), a3 = bytes_h2<0x4342>(w1);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < TERMS; ++e) mma16816(sc[j][nt], a0, a1, a2, a3, qf[nt][e][kk][0], qf[nt][e][kk][1]);
+            }
+        }
+        // the next unit's keys and scales, and the pages of the one after it
+        const float dk_u = dk, dv_u = dv;
+        pv = pv_next;
+        if (u + ST_WARPS < u1) {
+            const int pk = __shfl_sync(0xffffffffu, pv_next, g >> 1);
+            load_k(kr, u + ST_WARPS, pk);
+            load_d(pk, &dk, &dv);
+            pv_next = lookup(u + 2 * ST_WARPS);
+        }
+        // softmax: lane (g, t) has keys base + 4 j + 2 e of rows 2 t, 2 t + 1
+        const int kbase = u * ST_UNIT + 16 * (g >> 1) + (g & 1);
+        const bool whole = u * ST_UNIT + ST_UNIT - 1 <= first_pos && (p.window <= 0 || u * ST_UNIT > last_pos - p.window);
+        float dmax = dv_u;
+        dmax = fmaxf(dmax, __shfl_xor_sync(0xffffffffu, dmax, 8));
+        dmax = fmaxf(dmax, __shfl_xor_sync(0xffffffffu, dmax, 16));  // over g / 2
+        float dscale = 1.f;
+        if (dmax > D) {  // warp-uniform; with room, so that it happens rarely
+            dscale = D / (2.f * dmax);
+            D = 2.f * dmax;
+        }
+        const float rv = D > 0.f ? __fdiv_rn(dv_u, D) : dv_u;
+        bool moved = dscale != 1.f;
+        float alpha[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const float f = dk_u * qs[nt][q];
+                float mx = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float& x = sc[j][nt][2 * e + q];
+                        x *= f;
+                        if (!whole) {
+                            const int key = kbase + 4 * j + 2 * e;
+                            if (key > qp[nt][q] || (p.window > 0 && key <= qp[nt][q] - p.window)) x = -INFINITY;
+                        }
+                        mx = fmaxf(mx, x);
+                    }
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                const float mn = fmaxf(m[nt][q], mx);
+                const float a = mn == m[nt][q] ? 1.f : ex2(m[nt][q] - mn);
+                m[nt][q] = mn;
+                l[nt][q] *= a;
+                alpha[nt][q] = a * dscale;
+                moved |= a != 1.f;
+                const float sub = mn == -INFINITY ? 0.f : mn;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float& x = sc[j][nt][2 * e + q];
+                        const bool hidden = !whole && x == -INFINITY;  // leaves out what its scale holds, NaN too
+                        const float w = ex2(x - sub);
+                        l[nt][q] += w;
+                        x = hidden ? 0.f : w * rv;
+                    }
+            }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    o[nt][i][0] *= alpha[nt][0];
+                    o[nt][i][1] *= alpha[nt][1];
+                    o[nt][i][2] *= alpha[nt][0];
+                    o[nt][i][3] *= alpha[nt][1];
+                }
+        }
+        // O^T += V^T P^T
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t pf[NT][TERMS][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float a = sc[j][nt][2 * e], b = sc[j][nt][2 * e + 1];
+                    const uint32_t h = pack_h2(a, b);
+                    pf[nt][0][e] = transpose8(h);
+                    if constexpr (TERMS == 2) {
+                        const float2 f = unpack_h2(h);
+                        pf[nt][1][e] = transpose8(pack_h2(a - f.x, b - f.y));
+                    }
+                }
+#pragma unroll
+            for (int w = 0; w < VB / 4; ++w) {
+                uint32_t x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = vr[j][e].w[w] ^ 0x80808080u;
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {  // dims 4 w + 2 hf, + 1 of the lane's VB
+                    const uint32_t k01 = __byte_perm(x[0], x[1], hf ? 0x7362 : 0x5140), k23 = __byte_perm(x[2], x[3], hf ? 0x7362 : 0x5140);
+                    const uint32_t a0 = bytes_h2<0x4140>(k01), a1 = bytes_h2<0x4342>(k01), a2 = bytes_h2<0x4140>(k23), a3 = bytes_h2<0x4342>(k23);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < TERMS; ++e) mma16816(o[nt][2 * w + hf], a0, a1, a2, a3, pf[nt][e][0], pf[nt][e][1]);
+                }
+            }
+        }
+    }
+
+    // join the warps (in order), then write the row or the split's part
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            float x = l[nt][q];
+            x += __shfl_xor_sync(0xffffffffu, x, 4);
+            x += __shfl_xor_sync(0xffffffffu, x, 8);
+            x += __shfl_xor_sync(0xffffffffu, x, 16);
+            const int row = 8 * nt + 2 * t + q;
+            if (g == 0) {
+                s_ml[warp][row][0] = m[nt][q];
+                s_ml[warp][row][1] = x;
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                s_o[warp][row][VB * g + 2 * i] = o[nt][i][q] * D;
+                s_o[warp][row][VB * g + 2 * i + 1] = o[nt][i][2 + q] * D;
+            }
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < ROWS * HD; i += ST_THREADS) {
+        const int row = i / HD, d = i - row * HD, r = r0 + row;
+        if (r >= R) break;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < ST_WARPS; ++w) mx = fmaxf(mx, s_ml[w][row][0]);
+        float lt = 0.f, acc = 0.f;
+#pragma unroll
+        for (int w = 0; w < ST_WARPS; ++w) {
+            if (s_ml[w][row][1] == 0.f) continue;  // this warp saw no key of the row
+            const float a = s_ml[w][row][0] == mx ? 1.f : ex2(s_ml[w][row][0] - mx);
+            lt = fmaf(s_ml[w][row][1], a, lt);
+            acc = fmaf(s_o[w][row][d], a, acc);
+        }
+        if (p.splits == 1) {
+            static_cast<T*>(p.out)[((size_t)(sq.off + r / p.G) * p.H + kvh * p.G + r % p.G) * HD + d] =
+                from_f32<T>(lt == 0.f ? 0.f : __fdiv_rn(acc, lt));
+        } else {
+            const size_t at = ((size_t)item * p.splits + split) * ROWS + row;
+            p.part_o[at * HD + d] = acc;
+            if (d == 0) p.part_ml[at] = make_float2(mx, lt);
+        }
+    }
+}
+
+// Joins the splits of one row, in split order. One CTA per (item, row).
+template <class T, int HD>
+__global__ void __launch_bounds__(HD) kvb_attn_join_kernel(const StepParams p, int rows) {
+    const int row = blockIdx.x % rows, item = blockIdx.x / rows, d = threadIdx.x;
+    const int rg = item % p.groups, kvh = (item / p.groups) % p.c.hkv, s = item / p.groups / p.c.hkv;
+    const KvbSeq sq = kvb_seq(p.c, p.b, s);
+    const int R = sq.n * p.G, r = rg * rows + row;
+    if (r >= R || R > p.max_rows) return;
+    const size_t at = (size_t)item * p.splits * rows + row;
+    float mx = -INFINITY;
+    for (int i = 0; i < p.splits; ++i) mx = fmaxf(mx, p.part_ml[at + (size_t)i * rows].x);
+    float lt = 0.f, acc = 0.f;
+    for (int i = 0; i < p.splits; ++i) {
+        const float2 ml = p.part_ml[at + (size_t)i * rows];
+        if (ml.y == 0.f) continue;
+        const float a = ml.x == mx ? 1.f : ex2(ml.x - mx);
+        lt = fmaf(ml.y, a, lt);
+        acc = fmaf(p.part_o[(at + (size_t)i * rows) * HD + d], a, acc);
+    }
+    static_cast<T*>(p.out)[((size_t)(sq.off + r / p.G) * p.H + kvh * p.G + r % p.G) * HD + d] =
+        from_f32<T>(lt == 0.f ? 0.f : __fdiv_rn(acc, lt));
+}
+
+struct StepPlan {
+    int rows, groups, splits;
+    size_t ml_bytes, bytes;
+};
+
+// Splits along the keys until the GPU has several CTAs per resident slot, each
+// still with two units per warp.
+StepPlan step_plan(const at_ctx* ctx, const KvbDev& c, const KvbBatch& b, int64_t max_end, int n_heads, int window, int max_rows) {
+    const int G = n_heads / c.hkv;
+    const int most = (int)std::min<int64_t>((int64_t)b.max_tokens * G, max_rows);
+    StepPlan s;
+    s.rows = most <= 8 ? 8 : 16;
+    s.groups = (most + s.rows - 1) / s.rows;
+    const int64_t items = (int64_t)b.n_seqs * c.hkv * s.groups;
+    int64_t keys = max_end;
+    if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + b.max_tokens + ST_UNIT);
+    const int64_t units = (keys + ST_UNIT - 1) / ST_UNIT;
+    const int64_t want = (8 * 2 * ctx->num_sms + items - 1) / items;
+    s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, (units + 2 * ST_WARPS - 1) / (2 * ST_WARPS)));
+    AT_REQUIRE(items * s.splits <= INT32_MAX && items * s.rows <= INT32_MAX, AT_ERR_INVALID_ARG, "the batch is too large for one call");
+    s.ml_bytes = s.splits == 1 ? 0 : (size_t)items * s.splits * s.rows * sizeof(float2);
+    s.bytes = s.splits == 1 ? 0 : s.ml_bytes + (size_t)items * s.splits * s.rows * c.hd * sizeof(float);
+    return s;
+}
+
+template <class T, int HD>
+void launch_step(const StepParams& p, const StepPlan& s, cudaStream_t st) {
+    const int items = p.b.n_seqs * p.c.hkv * s.groups;
+    if (s.rows == 8) kvb_attn_step_kernel<T, HD, 1><<<items * s.splits, ST_THREADS, 0, st>>>(p);
+    else kvb_attn_step_kernel<T, HD, 2><<<items * s.splits, ST_THREADS, 0, st>>>(p);
+    AT_CUDA(cudaGetLastError());
+    if (s.splits > 1) {
+        kvb_attn_join_kernel<T, HD><<<items * s.rows, HD, 0, st>>>(p, s.rows);
+        AT_CUDA(cudaGetLastError());
+    }
+}
+
+constexpr int STEP_MAX_ROWS = 64;
+
 constexpr int SIMPLE_THREADS = 128;
 
 // One CTA per query token and query head: each warp walks every fourth key
@@ -22,13 +452,13 @@ constexpr int SIMPLE_THREADS = 128;
 template <class T, int HD>
 __global__ void __launch_bounds__(SIMPLE_THREADS) kvb_attn_simple_kernel(KvbDev c, KvbBatch b, const T* __restrict__ q,
                                                                          int64_t q_ts, int64_t q_hs, T* __restrict__ out, int H,
-                                                                         float scale, int window) {
+                                                                         float scale, int window, int min_rows) {
     constexpr int E = HD / 32, W = SIMPLE_THREADS / 32;
     __shared__ float s_m[W], s_l[W], s_o[W][HD];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int h = blockIdx.x % H, i = (blockIdx.x / H) % b.max_tokens, s = blockIdx.x / H / b.max_tokens;
     const KvbSeq sq = kvb_seq(c, b, s);
-    if (i >= sq.n) return;
+    if (i >= sq.n || sq.n * (H / c.hkv) <= min_rows) return;
     const int kvh = h / (H / c.hkv), pos = (int)sq.start + i;
     const int lo = window > 0 ? max(0, pos - window + 1) : 0;
     float qv[E], o[E];
@@ -72,6 +502,12 @@ __global__ void __launch_bounds__(SIMPLE_THREADS) kvb_attn_simple_kernel(KvbDev 
     }
 }
 
+// The step kernel serves every sequence of at most STEP_MAX_ROWS query rows
+// per KV head; it is left out when the host's sizes say that there is none.
+bool uses_step(const KvbBatch& b, int G) {
+    return b.max_tokens * G <= STEP_MAX_ROWS || (int64_t)b.n_seqs * b.max_tokens > b.n_tokens;
+}
+
 }  // namespace
 
 }  // namespace at
@@ -83,13 +519,15 @@ extern "C" {
 int at_kvb_attention_workspace(at_ctx* ctx, const at_kvb* cache, const at_token_batch* batch, int n_heads, int window,
                                size_t* bytes) {
     return guard([&] {
-        kvb_dev(ctx, cache, false);
-        kvb_batch(cache, batch);
+        AT_REQUIRE(ctx && cache && batch, AT_ERR_INVALID_ARG, "null argument");
         AT_REQUIRE(bytes, AT_ERR_INVALID_ARG, "null output");
         AT_REQUIRE(n_heads > 0 && n_heads % cache->n_kv_heads == 0, AT_ERR_INVALID_ARG,
                    "query heads must be a multiple of the KV heads");
-        (void)window;
+        const KvbDev c = kvb_dev(ctx, cache, false);
+        const KvbBatch b = kvb_batch(cache, batch);
         *bytes = 0;
+        if (b.n_seqs == 0 || b.max_tokens == 0) return;
+        if (uses_step(b, n_heads / c.hkv)) *bytes = step_plan(ctx, c, b, batch->max_end, n_heads, window, STEP_MAX_ROWS).bytes;
     });
 }
 
@@ -108,16 +546,27 @@ int at_kvb_attention(at_ctx* ctx, const at_kvb* cache, const at_token_batch* bat
         AT_REQUIRE(q && out, AT_ERR_INVALID_ARG, "null q or out");
         AT_REQUIRE(((uintptr_t)out & 15) == 0 && ((uintptr_t)q & (kvb_elem_bytes(dtype) - 1)) == 0, AT_ERR_INVALID_ARG,
                    "out must be 16-byte aligned, q aligned to its elements");
-        (void)workspace;
-        (void)workspace_bytes;
+        AT_CUDA(cudaSetDevice(ctx->device));
+        if (uses_step(b, n_heads / c.hkv)) {
+            const StepPlan s = step_plan(ctx, c, b, batch->max_end, n_heads, window, STEP_MAX_ROWS);
+            AT_REQUIRE(workspace_bytes >= s.bytes && (s.bytes == 0 || (workspace && ((uintptr_t)workspace & 15) == 0)), AT_ERR_INVALID_ARG,
+                       "attention: the workspace must be 16-byte aligned and hold at_kvb_attention_workspace bytes");
+            StepParams p{c, b, q, q_token_stride, q_head_stride, out, n_heads, n_heads / c.hkv, s.groups, s.splits, window, STEP_MAX_ROWS, scale,
+                         reinterpret_cast<float*>(static_cast<char*>(workspace) + s.ml_bytes), static_cast<float2*>(workspace)};
+            kvb_dispatch(dtype, [&](auto t) {
+                using T = decltype(t);
+                if (c.hd == 128) launch_step<T, 128>(p, s, ctx->stream);
+                else launch_step<T, 64>(p, s, ctx->stream);
+            });
+        }
+        if (b.max_tokens * (n_heads / c.hkv) <= STEP_MAX_ROWS) return;
         const int64_t grid = (int64_t)b.n_seqs * b.max_tokens * n_heads;
         AT_REQUIRE(grid <= INT32_MAX, AT_ERR_INVALID_ARG, "the batch is too large for one call");
-        AT_CUDA(cudaSetDevice(ctx->device));
         kvb_dispatch(dtype, [&](auto t) {
             using T = decltype(t);
             auto kern = c.hd == 128 ? kvb_attn_simple_kernel<T, 128> : kvb_attn_simple_kernel<T, 64>;
             kern<<<(int)grid, SIMPLE_THREADS, 0, ctx->stream>>>(c, b, static_cast<const T*>(q), q_token_stride, q_head_stride,
-                                                                static_cast<T*>(out), n_heads, scale, window);
+                                                                static_cast<T*>(out), n_heads, scale, window, STEP_MAX_ROWS);
         });
         AT_CUDA(cudaGetLastError());
     });
