@@ -71,20 +71,6 @@ namespace {
 constexpr int APPEND_THREADS = 256;
 constexpr uint32_t F32_INF = 0x7F800000u;
 
-// Eight consecutive elements as FP32; vec: p is 16-byte aligned.
-template <class T>
-__device__ __forceinline__ void load8(const T* __restrict__ p, bool vec, float* x) {
-    if (vec) {
-        alignas(16) T t[8];
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(t)[i] = reinterpret_cast<const uint4*>(p)[i];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(t[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(p[i]);
-    }
-}
 template <class T>
 __device__ __forceinline__ void store8(T* __restrict__ p, const float* x) {
     alignas(16) T t[8];
@@ -277,10 +263,7 @@ void launch_append(const KvbDev& c, const KvbBatch& b, const AppendSrc<T>& k, co
 
 template <class T>
 AppendSrc<T> append_src(const void* x, int64_t ts, int64_t hs) {
-    const int64_t per = 16 / (int64_t)sizeof(T);
-    AppendSrc<T> a{static_cast<const T*>(x), ts, hs, false};
-    a.vec = ((uintptr_t)x & 15) == 0 && ts % per == 0 && hs % per == 0;
-    return a;
+    return AppendSrc<T>{static_cast<const T*>(x), ts, hs, aligned_rows(x, (int)sizeof(T), ts, hs)};
 }
 
 }  // namespace

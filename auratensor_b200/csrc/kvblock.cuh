@@ -100,6 +100,26 @@ inline void kvb_dispatch(int dtype, F&& f) {
         default: fail(AT_ERR_UNSUPPORTED, "element type must be F32, F16 or BF16, got " + std::to_string(dtype));
     }
 }
+// Eight consecutive elements as FP32; vec: p is 16-byte aligned.
+template <class T>
+__device__ __forceinline__ void load8(const T* __restrict__ p, bool vec, float* x) {
+    if (vec) {
+        alignas(16) T t[8];
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(t)[i] = reinterpret_cast<const uint4*>(p)[i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(t[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(p[i]);
+    }
+}
+
 inline int kvb_elem_bytes(int dtype) { return dtype == AT_GGML_F32 ? 4 : 2; }
+
+// Whether every row of head_dim elements starts on a 16-byte boundary.
+inline bool aligned_rows(const void* x, int elem_bytes, int64_t token_stride, int64_t head_stride) {
+    return (((uintptr_t)x | (uintptr_t)(token_stride * elem_bytes) | (uintptr_t)(head_stride * elem_bytes)) & 15) == 0;
+}
 
 }  // namespace at

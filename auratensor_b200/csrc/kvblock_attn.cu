@@ -24,11 +24,15 @@ namespace {
 // are the M side of S^T = K Q^T, head dimensions the M side of O^T = V^T P^T.
 // Both A operands are built in registers from the int8 bytes as they come
 // from memory, exact in f16 (|q| <= 127), so K and V cross shared memory
-// nowhere: a warp's unit is 64 keys, 16-byte loads straight into the lanes
-// that multiply them. Which key or dimension a lane's bytes are is free, as
+// nowhere: a warp's unit is 32 or 64 keys, 16-byte loads straight into the
+// lanes that multiply them. A byte q becomes 1024 + 128 + q by one masked xor and
+// loses the offset in one packed subtraction; for F16/BF16 queries K skips the
+// subtraction: its f16 bits are q + 128 alone, a subnormal worth
+// (q + 128) 2^-24, and 128 sum(q_c) leaves the finished dot product (the
+// offset is 3 to 4 times the dot's own size, which costs FP32 sums two bits). Which key or dimension a lane's bytes are is free, as
 // long as both operands agree, and is chosen so that
-//   K: lane (g, t) holds 16 bytes of key rows 16 (g / 2) + 4 j + (g & 1), + 2;
-//   V: lane (g, t) holds HD / 8 bytes of keys 16 t + 4 j .. + 3;
+//   K: lane (g, t) holds 16-byte chunks of key rows 4 J (g / 2) + 4 j + (g & 1), + 2;
+//   V: lane (g, t) holds HD / 8 bytes of keys 4 J t + 4 j .. + 3 (J 16-key tiles per unit);
 //   the S^T accumulators, packed to f16 pairs and transposed by movmatrix,
 //   are the P^T operand.
 // tcgen05 would want the converted tiles in shared memory and 128 rows; here
@@ -40,7 +44,11 @@ namespace {
 // they stay in f16's range whatever the values' scale; O is kept in units of D.
 constexpr int ST_WARPS = 4;
 constexpr int ST_THREADS = 32 * ST_WARPS;
-constexpr int ST_UNIT = 64;
+// Keys of a warp's unit: 8 KB of K and V each at a time. At head_dim 128 a
+// unit of 64 keys needs 252 registers and leaves two warps per scheduler to
+// cover each other's latencies (64 sequences up to 8192 tokens: 163 us); 32
+// keys fit 168 registers and three.
+constexpr int st_unit(int hd) { return hd == 128 ? 32 : 64; }
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -52,14 +60,18 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {  // a in the low
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float2 unpack_h2(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
-// Two biased bytes (q + 128) of w, selected with 0x64 above each: 1024 + q + 128
-// as f16 pairs; minus 1152 is q, exactly.
-template <int SEL>
-__device__ __forceinline__ uint32_t bytes_h2(uint32_t w) {
-    const uint32_t m = __byte_perm(w, 0x64646464u, SEL);
-    const uint32_t c = 0x64806480u;
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&m), *reinterpret_cast<const __half2*>(&c));
-    return *reinterpret_cast<const uint32_t*>(&r);
+// Bytes 0 and 2 (odd: 1 and 3) of w as f16 pairs: q exactly, or, BIASED,
+// (q + 128) 2^-24.
+template <bool BIASED>
+__device__ __forceinline__ uint32_t bytes_h2(uint32_t w, bool odd) {
+    if (odd) w >>= 8;
+    if constexpr (BIASED) {
+        return (w & 0x00FF00FFu) ^ 0x00800080u;
+    } else {
+        const uint32_t m = (w & 0x00FF00FFu) ^ 0x64806480u, c = 0x64806480u;  // 1024 + 128 + q; 1152
+        const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&m), *reinterpret_cast<const __half2*>(&c));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
@@ -98,21 +110,33 @@ struct StepParams {
     int64_t q_ts, q_hs;
     void* out;
     int H, G, groups, splits, window, max_rows;  // groups: row groups of 8 NT; sequences above max_rows rows are skipped
+    int q_vec;                                   // q rows are 16-byte aligned
     float scale;
     float* part_o;   // [item][split][8 NT][HD]
     float2* part_ml; // [item][split][8 NT]
 };
 
+// Four outputs of a row: o / l (0 for a row that saw no key).
+template <class T>
+__device__ __forceinline__ void store_row4(T* out, float4 o, float l) {
+    const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+    alignas(16) T y[4] = {from_f32<T>(o.x * inv), from_f32<T>(o.y * inv), from_f32<T>(o.z * inv), from_f32<T>(o.w * inv)};
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(y);
+    else *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(y);
+}
+
 template <class T, int HD, int NT>
-__global__ void __launch_bounds__(ST_THREADS) kvb_attn_step_kernel(const StepParams p) {
+__global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 3 : 2) kvb_attn_step_kernel(const StepParams p) {
     constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
+    constexpr bool BIASED = TERMS == 1;
     constexpr int KS = HD / 16;    // k-steps of K Q^T
     constexpr int KC = HD / 64;    // 16-byte chunks of a key row per lane
     constexpr int MT = HD / 16;    // M tiles of V^T P^T
     constexpr int VB = HD / 8;     // bytes of a value row per lane
     constexpr int ROWS = 8 * NT;
+    constexpr int UNIT = st_unit(HD), J = UNIT / 16, SUB = 4 * J;  // SUB consecutive keys share a lane's page
     const KvbDev& c = p.c;
-    __shared__ float s_ml[ST_WARPS][ROWS][2];
+    __shared__ float s_ml[ST_WARPS][ROWS][2], s_w[ST_WARPS][ROWS], s_lt[ROWS], s_mx[ROWS];
     __shared__ float s_o[ST_WARPS][ROWS][HD];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int item = blockIdx.x / p.splits, split = blockIdx.x - item * p.splits;
@@ -123,46 +147,58 @@ __global__ void __launch_bounds__(ST_THREADS) kvb_attn_step_kernel(const StepPar
     const int start = (int)sq.start;
     const int first_pos = start + r0 / p.G, last_pos = start + (min(R, r0 + ROWS) - 1) / p.G;
     const int lo = p.window > 0 ? max(0, first_pos - p.window + 1) : 0, hi = last_pos + 1;
-    const int u_lo = lo / ST_UNIT, nu = (hi - 1) / ST_UNIT + 1 - u_lo;
+    const int u_lo = lo / UNIT, nu = (hi - 1) / UNIT + 1 - u_lo;
     const int u0 = u_lo + (int)((int64_t)nu * split / p.splits), u1 = u_lo + (int)((int64_t)nu * (split + 1) / p.splits);
 
     // queries: row g of each tile, 4 dims per k-step
     uint32_t qf[NT][TERMS][KS][2];
     float qs[NT][2];  // score factors of rows 2 t, 2 t + 1 (log2 units)
+    float qb[NT][2];  // 128 sum(q_c) of the same rows (the K offset)
     int qp[NT][2];    // their positions (padding rows: -1, they see nothing)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int r = r0 + 8 * nt + g;
         float x[KC][16];
         float top = 0.f;
+        if (r < R) {
+            const T* row = static_cast<const T*>(p.q) + (int64_t)(sq.off + r / p.G) * p.q_ts + (int64_t)(kvh * p.G + r % p.G) * p.q_hs + 16 * t;
+#pragma unroll
+            for (int cc = 0; cc < KC; ++cc) {
+                load8<T>(row + 64 * cc, p.q_vec, x[cc]);
+                load8<T>(row + 64 * cc + 8, p.q_vec, x[cc] + 8);
+            }
+        } else {
+#pragma unroll
+            for (int cc = 0; cc < KC; ++cc)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[cc][i] = 0.f;
+        }
 #pragma unroll
         for (int cc = 0; cc < KC; ++cc)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                x[cc][i] = r < R ? to_f32<T>(static_cast<const T*>(p.q)[(int64_t)(sq.off + r / p.G) * p.q_ts +
-                                                                      (int64_t)(kvh * p.G + r % p.G) * p.q_hs + 64 * cc + 16 * t + i])
-                                 : 0.f;
-                top = fmaxf(top, fabsf(x[cc][i]));
-            }
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(x[cc][i]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const float rs = row_scale(top);
+        float sum = 0.f;
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk)
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                const float a0 = x[kk >> 2][4 * (kk & 3) + 2 * b] * rs, a1 = x[kk >> 2][4 * (kk & 3) + 2 * b + 1] * rs;
+                const float a0 = x[kk >> 2][4 * (kk & 3) + b] * rs, a1 = x[kk >> 2][4 * (kk & 3) + b + 2] * rs;
                 const uint32_t hi2 = pack_h2(a0, a1);
+                const float2 h = unpack_h2(hi2);
                 qf[nt][0][kk][b] = hi2;
-                if constexpr (TERMS == 2) {
-                    const float2 h = unpack_h2(hi2);
-                    qf[nt][1][kk][b] = pack_h2(a0 - h.x, a1 - h.y);
-                }
+                sum += h.x + h.y;
+                if constexpr (TERMS == 2) qf[nt][1][kk][b] = pack_h2(a0 - h.x, a1 - h.y);
             }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         const float f = p.scale * 1.44269504088896341f / rs;  // exact division: rs is a power of two
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             qs[nt][e] = __shfl_sync(0xffffffffu, f, (2 * t + e) * 4);
+            qb[nt][e] = 128.f * __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4);
             const int rr = r0 + 8 * nt + 2 * t + e;
             qp[nt][e] = rr < R ? start + rr / p.G : -1;
         }
@@ -179,12 +215,12 @@ __global__ void __launch_bounds__(ST_THREADS) kvb_attn_step_kernel(const StepPar
     }
 
     // page of this lane's sub-block t of a unit (-2: past the last key, -1: outside the pool)
-    auto lookup = [&](int u) { return (u < u1 && u * ST_UNIT + 16 * t < hi) ? kvb_page(c, sq.slot, (u * ST_UNIT + 16 * t) >> c.lb) : -2; };
+    auto lookup = [&](int u) { return (u < u1 && u * UNIT + SUB * t < hi) ? kvb_page(c, sq.slot, (u * UNIT + SUB * t) >> c.lb) : -2; };
     const int bmask = (1 << c.lb) - 1;
-    auto load_k = [&](Bytes<16> (&kr)[4][2][KC], int u, int pk) {  // pk: page of sub-block g / 2
-        const int8_t* base = c.k + ((((size_t)max(pk, 0) * c.hkv + kvh) << c.lb) + ((u * ST_UNIT + 16 * (g >> 1)) & bmask)) * HD + 16 * t;
+    auto load_k = [&](Bytes<16> (&kr)[J][2][KC], int u, int pk) {  // pk: page of sub-block g / 2
+        const int8_t* base = c.k + ((((size_t)max(pk, 0) * c.hkv + kvh) << c.lb) + ((u * UNIT + SUB * (g >> 1)) & bmask)) * HD + 16 * t;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < J; ++j)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -198,7 +234,7 @@ __global__ void __launch_bounds__(ST_THREADS) kvb_attn_step_kernel(const StepPar
 
     int u = u0 + warp;
     int pv = lookup(u), pv_next = lookup(u + ST_WARPS);
-    Bytes<16> kr[4][2][KC];
+    Bytes<16> kr[J][2][KC];
     float dk, dv;
     {
         const int pk = __shfl_sync(0xffffffffu, pv, g >> 1);
@@ -207,23 +243,24 @@ __global__ void __launch_bounds__(ST_THREADS) kvb_attn_step_kernel(const StepPar
     }
     for (; u < u1; u += ST_WARPS) {
         // the values' bytes are asked for before the keys are multiplied
-        Bytes<VB> vr[4][4];
+        Bytes<VB> vr[J][4];
         {
-            const int8_t* base = c.v + ((((size_t)max(pv, 0) * c.hkv + kvh) << c.lb) + ((u * ST_UNIT + 16 * t) & bmask)) * HD + VB * g;
+            const int8_t* base = c.v + ((((size_t)max(pv, 0) * c.hkv + kvh) << c.lb) + ((u * UNIT + SUB * t) & bmask)) * HD + VB * g;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < J; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) ld_bytes(vr[j][e], base + (4 * j + e) * HD);
         }
-        float sc[4][NT][4];
+        float sc[J][NT][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < J; ++j) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) sc[j][nt][0] = sc[j][nt][1] = sc[j][nt][2] = sc[j][nt][3] = 0.f;
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk) {
-                const uint32_t w0 = kr[j][0][kk >> 2].w[kk & 3] ^ 0x80808080u, w1 = kr[j][1][kk >> 2].w[kk & 3] ^ 0x80808080u;
-                const uint32_t a0 = bytes_h2<0x4140>(w0), a1 = bytes_h2<0x4140>(w1), a2 = bytes_h2<0x4342>(w0), a3 = bytes_h2<0x4342>(w1);
+                const uint32_t w0 = kr[j][0][kk >> 2].w[kk & 3], w1 = kr[j][1][kk >> 2].w[kk & 3];
+                const uint32_t a0 = bytes_h2<BIASED>(w0, false), a1 = bytes_h2<BIASED>(w1, false);
+                const uint32_t a2 = bytes_h2<BIASED>(w0, true), a3 = bytes_h2<BIASED>(w1, true);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -240,8 +277,8 @@ __global__ void __launch_bounds__(ST_THREADS) kvb_attn_step_kernel(const StepPar
             pv_next = lookup(u + 2 * ST_WARPS);
         }
         // softmax: lane (g, t) has keys base + 4 j + 2 e of rows 2 t, 2 t + 1
-        const int kbase = u * ST_UNIT + 16 * (g >> 1) + (g & 1);
-        const bool whole = u * ST_UNIT + ST_UNIT - 1 <= first_pos && (p.window <= 0 || u * ST_UNIT > last_pos - p.window);
+        const int kbase = u * UNIT + SUB * (g >> 1) + (g & 1);
+        const bool whole = u * UNIT + UNIT - 1 <= first_pos && (p.window <= 0 || u * UNIT > last_pos - p.window);
         float dmax = dv_u;
         dmax = fmaxf(dmax, __shfl_xor_sync(0xffffffffu, dmax, 8));
         dmax = fmaxf(dmax, __shfl_xor_sync(0xffffffffu, dmax, 16));  // over g / 2
@@ -257,20 +294,23 @@ __global__ void __launch_bounds__(ST_THREADS) kvb_attn_step_kernel(const StepPar
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                const float f = dk_u * qs[nt][q];
+                const float f0 = dk_u * qs[nt][q], f = BIASED ? f0 * 0x1p24f : f0, off = BIASED ? -qb[nt][q] * f0 : 0.f;
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) sc[j][nt][2 * e + q] = fmaf(sc[j][nt][2 * e + q], f, off);
+                if (!whole) {
+#pragma unroll
+                    for (int j = 0; j < J; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int key = kbase + 4 * j + 2 * e;
+                            if (key > qp[nt][q] || (p.window > 0 && key <= qp[nt][q] - p.window)) sc[j][nt][2 * e + q] = -INFINITY;
+                        }
+                }
                 float mx = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float& x = sc[j][nt][2 * e + q];
-                        x *= f;
-                        if (!whole) {
-                            const int key = kbase + 4 * j + 2 * e;
-                            if (key > qp[nt][q] || (p.window > 0 && key <= qp[nt][q] - p.window)) x = -INFINITY;
-                        }
-                        mx = fmaxf(mx, x);
-                    }
+                for (int j = 0; j < J; ++j) mx = fmaxf(mx, fmaxf(sc[j][nt][q], sc[j][nt][2 + q]));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -281,17 +321,31 @@ __global__ void __launch_bounds__(ST_THREADS) kvb_attn_step_kernel(const StepPar
                 alpha[nt][q] = a * dscale;
                 moved |= a != 1.f;
                 const float sub = mn == -INFINITY ? 0.f : mn;
+                float sum = 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < J; ++j)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         float& x = sc[j][nt][2 * e + q];
-                        const bool hidden = !whole && x == -INFINITY;  // leaves out what its scale holds, NaN too
-                        const float w = ex2(x - sub);
-                        l[nt][q] += w;
-                        x = hidden ? 0.f : w * rv;
+                        x = ex2(x - sub);
+                        sum += x;
+                        x *= rv;
                     }
+                l[nt][q] += sum;
             }
+        if (!whole) {  // a hidden key has no weight whatever its block's scale holds (0 NaN is NaN)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int j = 0; j < J; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int key = kbase + 4 * j + 2 * e;
+                            if (key > qp[nt][q] || (p.window > 0 && key <= qp[nt][q] - p.window)) sc[j][nt][2 * e + q] = 0.f;
+                        }
+        }
         if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -305,7 +359,7 @@ __global__ void __launch_bounds__(ST_THREADS) kvb_attn_step_kernel(const StepPar
         }
         // O^T += V^T P^T
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < J; ++j) {
             uint32_t pf[NT][TERMS][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -323,11 +377,12 @@ __global__ void __launch_bounds__(ST_THREADS) kvb_attn_step_kernel(const StepPar
             for (int w = 0; w < VB / 4; ++w) {
                 uint32_t x[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = vr[j][e].w[w] ^ 0x80808080u;
+                for (int e = 0; e < 4; ++e) x[e] = vr[j][e].w[w];
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {  // dims 4 w + 2 hf, + 1 of the lane's VB
-                    const uint32_t k01 = __byte_perm(x[0], x[1], hf ? 0x7362 : 0x5140), k23 = __byte_perm(x[2], x[3], hf ? 0x7362 : 0x5140);
-                    const uint32_t a0 = bytes_h2<0x4140>(k01), a1 = bytes_h2<0x4342>(k01), a2 = bytes_h2<0x4140>(k23), a3 = bytes_h2<0x4342>(k23);
+                    const uint32_t k01 = __byte_perm(x[0], x[1], hf ? 0x7632 : 0x5410), k23 = __byte_perm(x[2], x[3], hf ? 0x7632 : 0x5410);
+                    const uint32_t a0 = bytes_h2<false>(k01, false), a1 = bytes_h2<false>(k01, true);
+                    const uint32_t a2 = bytes_h2<false>(k23, false), a3 = bytes_h2<false>(k23, true);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -358,52 +413,86 @@ __global__ void __launch_bounds__(ST_THREADS) kvb_attn_step_kernel(const StepPar
             }
         }
     __syncthreads();
-    for (int i = threadIdx.x; i < ROWS * HD; i += ST_THREADS) {
-        const int row = i / HD, d = i - row * HD, r = r0 + row;
-        if (r >= R) break;
-        float mx = -INFINITY;
+    if (threadIdx.x < ROWS) {
+        const int row = threadIdx.x;
+        float mx = -INFINITY, lt = 0.f;
 #pragma unroll
         for (int w = 0; w < ST_WARPS; ++w) mx = fmaxf(mx, s_ml[w][row][0]);
-        float lt = 0.f, acc = 0.f;
 #pragma unroll
         for (int w = 0; w < ST_WARPS; ++w) {
-            if (s_ml[w][row][1] == 0.f) continue;  // this warp saw no key of the row
-            const float a = s_ml[w][row][0] == mx ? 1.f : ex2(s_ml[w][row][0] - mx);
-            lt = fmaf(s_ml[w][row][1], a, lt);
-            acc = fmaf(s_o[w][row][d], a, acc);
+            const float lw = s_ml[w][row][1], a = s_ml[w][row][0] == mx ? 1.f : ex2(s_ml[w][row][0] - mx);
+            s_w[w][row] = lw == 0.f ? 0.f : a;  // 0: this warp saw no key of the row
+            if (lw != 0.f) lt = fmaf(lw, a, lt);
+        }
+        s_lt[row] = lt;
+        s_mx[row] = mx;
+    }
+    __syncthreads();
+    const int rows = min(ROWS, R - r0);
+    for (int i = threadIdx.x; i < rows * (HD / 4); i += ST_THREADS) {
+        const int row = i / (HD / 4), d = 4 * (i % (HD / 4)), r = r0 + row;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < ST_WARPS; ++w) {
+            const float a = s_w[w][row];
+            if (a == 0.f) continue;
+            const float4 x = *reinterpret_cast<const float4*>(&s_o[w][row][d]);
+            acc.x = fmaf(x.x, a, acc.x);
+            acc.y = fmaf(x.y, a, acc.y);
+            acc.z = fmaf(x.z, a, acc.z);
+            acc.w = fmaf(x.w, a, acc.w);
         }
         if (p.splits == 1) {
-            static_cast<T*>(p.out)[((size_t)(sq.off + r / p.G) * p.H + kvh * p.G + r % p.G) * HD + d] =
-                from_f32<T>(lt == 0.f ? 0.f : __fdiv_rn(acc, lt));
+            store_row4<T>(static_cast<T*>(p.out) + ((size_t)(sq.off + r / p.G) * p.H + kvh * p.G + r % p.G) * HD + d, acc, s_lt[row]);
         } else {
             const size_t at = ((size_t)item * p.splits + split) * ROWS + row;
-            p.part_o[at * HD + d] = acc;
-            if (d == 0) p.part_ml[at] = make_float2(mx, lt);
+            *reinterpret_cast<float4*>(p.part_o + at * HD + d) = acc;
+            if (d == 0) p.part_ml[at] = make_float2(s_mx[row], s_lt[row]);
         }
     }
 }
 
-// Joins the splits of one row, in split order. One CTA per (item, row).
+// Joins the splits of a row, in split order: HD / 4 threads per row. The
+// weights of up to 32 splits are found by the lanes of a warp together.
 template <class T, int HD>
-__global__ void __launch_bounds__(HD) kvb_attn_join_kernel(const StepParams p, int rows) {
-    const int row = blockIdx.x % rows, item = blockIdx.x / rows, d = threadIdx.x;
+__global__ void __launch_bounds__(128) kvb_attn_join_kernel(const StepParams p, int rows, int total) {
+    constexpr int TPR = HD / 4;  // threads per row: 16 or 32
+    const int lane = threadIdx.x % TPR;
+    const uint32_t mask = TPR == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);
+    const int gr = blockIdx.x * (128 / TPR) + threadIdx.x / TPR;
+    if (gr >= total) return;
+    const int row = gr % rows, item = gr / rows;
     const int rg = item % p.groups, kvh = (item / p.groups) % p.c.hkv, s = item / p.groups / p.c.hkv;
     const KvbSeq sq = kvb_seq(p.c, p.b, s);
     const int R = sq.n * p.G, r = rg * rows + row;
     if (r >= R || R > p.max_rows) return;
     const size_t at = (size_t)item * p.splits * rows + row;
     float mx = -INFINITY;
-    for (int i = 0; i < p.splits; ++i) mx = fmaxf(mx, p.part_ml[at + (size_t)i * rows].x);
-    float lt = 0.f, acc = 0.f;
-    for (int i = 0; i < p.splits; ++i) {
-        const float2 ml = p.part_ml[at + (size_t)i * rows];
-        if (ml.y == 0.f) continue;
-        const float a = ml.x == mx ? 1.f : ex2(ml.x - mx);
-        lt = fmaf(ml.y, a, lt);
-        acc = fmaf(p.part_o[(at + (size_t)i * rows) * HD + d], a, acc);
+    for (int i = lane; i < p.splits; i += TPR) mx = fmaxf(mx, p.part_ml[at + (size_t)i * rows].x);
+#pragma unroll
+    for (int o = TPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(mask, mx, o, TPR));
+    float lt = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < p.splits; i0 += TPR) {
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (i0 + lane < p.splits) ml = p.part_ml[at + (size_t)(i0 + lane) * rows];
+        const float a = ml.y == 0.f ? 0.f : ml.x == mx ? 1.f : ex2(ml.x - mx);
+        lt += ml.y == 0.f ? 0.f : ml.y * a;
+        const int n = min(TPR, p.splits - i0);
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+            const float4 x = *reinterpret_cast<const float4*>(p.part_o + (at + (size_t)(i0 + i) * rows) * HD + 4 * lane);
+            const float w = __shfl_sync(mask, a, i, TPR);
+            if (w == 0.f) continue;
+            acc.x = fmaf(x.x, w, acc.x);
+            acc.y = fmaf(x.y, w, acc.y);
+            acc.z = fmaf(x.z, w, acc.z);
+            acc.w = fmaf(x.w, w, acc.w);
+        }
     }
-    static_cast<T*>(p.out)[((size_t)(sq.off + r / p.G) * p.H + kvh * p.G + r % p.G) * HD + d] =
-        from_f32<T>(lt == 0.f ? 0.f : __fdiv_rn(acc, lt));
+#pragma unroll
+    for (int o = TPR / 2; o > 0; o >>= 1) lt += __shfl_xor_sync(mask, lt, o, TPR);
+    store_row4<T>(static_cast<T*>(p.out) + ((size_t)(sq.off + r / p.G) * p.H + kvh * p.G + r % p.G) * HD + 4 * lane, acc, lt);
 }
 
 struct StepPlan {
@@ -411,8 +500,12 @@ struct StepPlan {
     size_t ml_bytes, bytes;
 };
 
-// Splits along the keys until the GPU has several CTAs per resident slot, each
-// still with two units per warp.
+// Splits along the keys. Three CTAs are resident per SM (two for 16 rows).
+// Fewer items than that: as many splits as fill the GPU once (more only
+// lengthen the join: one sequence of 131072 tokens, 8 KV heads of 64: 40 us
+// at 1 wave, 51 at 3). More items: several waves, because sequences differ in
+// length (64 sequences of 4096 to 8192 tokens: 192 us unsplit at 1.2 waves,
+// 153 at 3.5). A split keeps at least one unit per warp.
 StepPlan step_plan(const at_ctx* ctx, const KvbDev& c, const KvbBatch& b, int64_t max_end, int n_heads, int window, int max_rows) {
     const int G = n_heads / c.hkv;
     const int most = (int)std::min<int64_t>((int64_t)b.max_tokens * G, max_rows);
@@ -421,10 +514,11 @@ StepPlan step_plan(const at_ctx* ctx, const KvbDev& c, const KvbBatch& b, int64_
     s.groups = (most + s.rows - 1) / s.rows;
     const int64_t items = (int64_t)b.n_seqs * c.hkv * s.groups;
     int64_t keys = max_end;
-    if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + b.max_tokens + ST_UNIT);
-    const int64_t units = (keys + ST_UNIT - 1) / ST_UNIT;
-    const int64_t want = (8 * 2 * ctx->num_sms + items - 1) / items;
-    s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, (units + 2 * ST_WARPS - 1) / (2 * ST_WARPS)));
+    if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + b.max_tokens + 64);
+    const int64_t units = (keys + st_unit(c.hd) - 1) / st_unit(c.hd);
+    const int64_t slots = (s.rows == 8 ? 3 : 2) * (int64_t)ctx->num_sms;
+    const int64_t want = items >= slots ? (7 * slots / 2 + items - 1) / items : slots / items;
+    s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, (units + ST_WARPS - 1) / ST_WARPS));
     AT_REQUIRE(items * s.splits <= INT32_MAX && items * s.rows <= INT32_MAX, AT_ERR_INVALID_ARG, "the batch is too large for one call");
     s.ml_bytes = s.splits == 1 ? 0 : (size_t)items * s.splits * s.rows * sizeof(float2);
     s.bytes = s.splits == 1 ? 0 : s.ml_bytes + (size_t)items * s.splits * s.rows * c.hd * sizeof(float);
@@ -438,7 +532,8 @@ void launch_step(const StepParams& p, const StepPlan& s, cudaStream_t st) {
     else kvb_attn_step_kernel<T, HD, 2><<<items * s.splits, ST_THREADS, 0, st>>>(p);
     AT_CUDA(cudaGetLastError());
     if (s.splits > 1) {
-        kvb_attn_join_kernel<T, HD><<<items * s.rows, HD, 0, st>>>(p, s.rows);
+        const int total = items * s.rows, per = 128 / (HD / 4);
+        kvb_attn_join_kernel<T, HD><<<(total + per - 1) / per, 128, 0, st>>>(p, s.rows, total);
         AT_CUDA(cudaGetLastError());
     }
 }
@@ -551,8 +646,9 @@ int at_kvb_attention(at_ctx* ctx, const at_kvb* cache, const at_token_batch* bat
             const StepPlan s = step_plan(ctx, c, b, batch->max_end, n_heads, window, STEP_MAX_ROWS);
             AT_REQUIRE(workspace_bytes >= s.bytes && (s.bytes == 0 || (workspace && ((uintptr_t)workspace & 15) == 0)), AT_ERR_INVALID_ARG,
                        "attention: the workspace must be 16-byte aligned and hold at_kvb_attention_workspace bytes");
-            StepParams p{c, b, q, q_token_stride, q_head_stride, out, n_heads, n_heads / c.hkv, s.groups, s.splits, window, STEP_MAX_ROWS, scale,
+            StepParams p{c, b, q, q_token_stride, q_head_stride, out, n_heads, n_heads / c.hkv, s.groups, s.splits, window, STEP_MAX_ROWS, 0, scale,
                          reinterpret_cast<float*>(static_cast<char*>(workspace) + s.ml_bytes), static_cast<float2*>(workspace)};
+            p.q_vec = aligned_rows(q, kvb_elem_bytes(dtype), q_token_stride, q_head_stride);
             kvb_dispatch(dtype, [&](auto t) {
                 using T = decltype(t);
                 if (c.hd == 128) launch_step<T, 128>(p, s, ctx->stream);
