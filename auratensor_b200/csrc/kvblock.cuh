@@ -15,6 +15,7 @@ namespace at {
 
 // Bits of the cache's status word (at_kvb.status).
 constexpr int KVB_BAD_SEQ = 1;    // a slot, start or offset outside its range: the sequence was skipped
+constexpr int KVB_STALLED = 4;    // a bounded wait inside a kernel ran out: its output is not valid
 constexpr int KVB_BAD_BLOCK = 2;  // a block-table entry outside the pool: reads give NaN, writes are dropped
 
 struct KvbDev {

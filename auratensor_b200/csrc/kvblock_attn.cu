@@ -11,6 +11,7 @@
 #include <string>
 
 #include "kvblock.cuh"
+#include "kvblock_attn.cuh"
 
 namespace at {
 
@@ -39,9 +40,10 @@ namespace {
 // there are 8 or 16 and the time goes to the K and V bytes.
 // FP32 queries are split into two f16 parts (22 bits), and so are the weights;
 // F16/BF16 queries are exact in one (each row is scaled by a power of two
-// into f16's range) and their weights are rounded once to 11 bits. Weights
-// carry d_v relative to a running reference D (at least every d_v so far), so
-// they stay in f16's range whatever the values' scale; O is kept in units of D.
+// into f16's range) and their weights are rounded once to 11 bits. The values'
+// scale is part of the weights' exponent: with t_j = s_j + log2 d_v(j) and m
+// their running maximum, P_j = 2^(t_j - m) <= 1 fills f16's range whatever the
+// blocks' scales are; out = sum P_j v8_j / sum P_j / d_v(j).
 constexpr int ST_WARPS = 4;
 constexpr int ST_THREADS = 32 * ST_WARPS;
 // Keys of a warp's unit: 8 KB of K and V each at a time. At head_dim 128 a
@@ -50,29 +52,6 @@ constexpr int ST_THREADS = 32 * ST_WARPS;
 // keys fit 168 registers and three.
 constexpr int st_unit(int hd) { return hd == 128 ? 32 : 64; }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t pack_h2(float a, float b) {  // a in the low half
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 unpack_h2(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
-// Bytes 0 and 2 (odd: 1 and 3) of w as f16 pairs: q exactly, or, BIASED,
-// (q + 128) 2^-24.
-template <bool BIASED>
-__device__ __forceinline__ uint32_t bytes_h2(uint32_t w, bool odd) {
-    if (odd) w >>= 8;
-    if constexpr (BIASED) {
-        return (w & 0x00FF00FFu) ^ 0x00800080u;
-    } else {
-        const uint32_t m = (w & 0x00FF00FFu) ^ 0x64806480u, c = 0x64806480u;  // 1024 + 128 + q; 1152
-        const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&m), *reinterpret_cast<const __half2*>(&c));
-        return *reinterpret_cast<const uint32_t*>(&r);
-    }
-}
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -95,12 +74,6 @@ __device__ __forceinline__ void ld_bytes(Bytes<16>& b, const int8_t* p) {
 }
 __device__ __forceinline__ void ld_bytes(Bytes<8>& b, const int8_t* p) {
     asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(b.w[0]), "=r"(b.w[1]) : "l"(p));
-}
-
-// Power of two that brings a row whose largest |x| is `top` to [512, 1024).
-__device__ __forceinline__ float row_scale(float top) {
-    const int e = (int)(__float_as_uint(top) >> 23) - 127;  // -127: zero or subnormal
-    return __uint_as_float((uint32_t)(127 + min(9 - e, 126)) << 23);
 }
 
 struct StepParams {
@@ -205,7 +178,7 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 3 : 2) kvb_attn_step_ker
     }
 
     float o[NT][MT][4];
-    float m[NT][2], l[NT][2], D = 0.f;
+    float m[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -279,16 +252,9 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 3 : 2) kvb_attn_step_ker
         // softmax: lane (g, t) has keys base + 4 j + 2 e of rows 2 t, 2 t + 1
         const int kbase = u * UNIT + SUB * (g >> 1) + (g & 1);
         const bool whole = u * UNIT + UNIT - 1 <= first_pos && (p.window <= 0 || u * UNIT > last_pos - p.window);
-        float dmax = dv_u;
-        dmax = fmaxf(dmax, __shfl_xor_sync(0xffffffffu, dmax, 8));
-        dmax = fmaxf(dmax, __shfl_xor_sync(0xffffffffu, dmax, 16));  // over g / 2
-        float dscale = 1.f;
-        if (dmax > D) {  // warp-uniform; with room, so that it happens rarely
-            dscale = D / (2.f * dmax);
-            D = 2.f * dmax;
-        }
-        const float rv = D > 0.f ? __fdiv_rn(dv_u, D) : dv_u;
-        bool moved = dscale != 1.f;
+        float lv, iv, mv;
+        value_scale<!BIASED>(dv_u, &lv, &iv, &mv);
+        bool moved = false;
         float alpha[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -311,6 +277,7 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 3 : 2) kvb_attn_step_ker
                 float mx = -INFINITY;
 #pragma unroll
                 for (int j = 0; j < J; ++j) mx = fmaxf(mx, fmaxf(sc[j][nt][q], sc[j][nt][2 + q]));
+                mx += lv;
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -318,26 +285,14 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 3 : 2) kvb_attn_step_ker
                 const float a = mn == m[nt][q] ? 1.f : ex2(m[nt][q] - mn);
                 m[nt][q] = mn;
                 l[nt][q] *= a;
-                alpha[nt][q] = a * dscale;
+                alpha[nt][q] = a;
                 moved |= a != 1.f;
-                const float sub = mn == -INFINITY ? 0.f : mn;
-                float sum = 0.f;
+                const float sub = mn == -INFINITY ? 0.f : mn - lv;
 #pragma unroll
                 for (int j = 0; j < J; ++j)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float& x = sc[j][nt][2 * e + q];
-                        x = ex2(x - sub);
-                        sum += x;
-                        x *= rv;
-                    }
-                l[nt][q] += sum;
-            }
-        if (!whole) {  // a hidden key has no weight whatever its block's scale holds (0 NaN is NaN)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
+                    for (int e = 0; e < 2; ++e) sc[j][nt][2 * e + q] = ex2(sc[j][nt][2 * e + q] - sub);
+                auto hide = [&] {  // a hidden key has no weight whatever its block's scales hold (0 NaN is NaN)
 #pragma unroll
                     for (int j = 0; j < J; ++j)
 #pragma unroll
@@ -345,7 +300,20 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 3 : 2) kvb_attn_step_ker
                             const int key = kbase + 4 * j + 2 * e;
                             if (key > qp[nt][q] || (p.window > 0 && key <= qp[nt][q] - p.window)) sc[j][nt][2 * e + q] = 0.f;
                         }
-        }
+                };
+                if (!whole) hide();
+                float sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < J; ++j) sum += sc[j][nt][q] + sc[j][nt][2 + q];
+                if (sum != 0.f) l[nt][q] = fmaf(sum, iv, l[nt][q]);
+                if constexpr (!BIASED) {
+#pragma unroll
+                    for (int j = 0; j < J; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) sc[j][nt][2 * e + q] *= mv;
+                    if (!whole) hide();
+                }
+            }
         if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -408,8 +376,8 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 3 : 2) kvb_attn_step_ker
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                s_o[warp][row][VB * g + 2 * i] = o[nt][i][q] * D;
-                s_o[warp][row][VB * g + 2 * i + 1] = o[nt][i][2 + q] * D;
+                s_o[warp][row][VB * g + 2 * i] = o[nt][i][q];
+                s_o[warp][row][VB * g + 2 * i + 1] = o[nt][i][2 + q];
             }
         }
     __syncthreads();
@@ -540,63 +508,6 @@ void launch_step(const StepParams& p, const StepPlan& s, cudaStream_t st) {
 
 constexpr int STEP_MAX_ROWS = 64;
 
-constexpr int SIMPLE_THREADS = 128;
-
-// One CTA per query token and query head: each warp walks every fourth key
-// with the lanes across the head dimension, then the warps are joined.
-template <class T, int HD>
-__global__ void __launch_bounds__(SIMPLE_THREADS) kvb_attn_simple_kernel(KvbDev c, KvbBatch b, const T* __restrict__ q,
-                                                                         int64_t q_ts, int64_t q_hs, T* __restrict__ out, int H,
-                                                                         float scale, int window, int min_rows) {
-    constexpr int E = HD / 32, W = SIMPLE_THREADS / 32;
-    __shared__ float s_m[W], s_l[W], s_o[W][HD];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int h = blockIdx.x % H, i = (blockIdx.x / H) % b.max_tokens, s = blockIdx.x / H / b.max_tokens;
-    const KvbSeq sq = kvb_seq(c, b, s);
-    if (i >= sq.n || sq.n * (H / c.hkv) <= min_rows) return;
-    const int kvh = h / (H / c.hkv), pos = (int)sq.start + i;
-    const int lo = window > 0 ? max(0, pos - window + 1) : 0;
-    float qv[E], o[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        qv[e] = to_f32<T>(q[(int64_t)(sq.off + i) * q_ts + (int64_t)h * q_hs + lane * E + e]) * scale;
-        o[e] = 0.f;
-    }
-    float m = -INFINITY, l = 0.f;
-    for (int j = lo + warp; j <= pos; j += W) {
-        const int page = kvb_page(c, sq.slot, j >> c.lb);
-        const size_t ph = (size_t)max(page, 0) * c.hkv + kvh;
-        const float dk = page < 0 ? __uint_as_float(0x7FC00000u) : c.ks[ph], dv = page < 0 ? dk : c.vs[ph];
-        const size_t at = ((ph << c.lb) + (j & ((1 << c.lb) - 1))) * HD + lane * E;
-        float dot = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) dot = fmaf(qv[e], (float)c.k[at + e], dot);
-        const float sc = warp_sum(dot) * dk;
-        const float mn = fmaxf(m, sc);
-        const float a = mn == -INFINITY ? 1.f : expf(m - mn), p = expf(sc - mn);
-        l = fmaf(l, a, p);
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(o[e], a, p * dv * (float)c.v[at + e]);
-        m = mn;
-    }
-    if (lane == 0) {
-        s_m[warp] = m;
-        s_l[warp] = l;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
-    __syncthreads();
-    float mx = -INFINITY;
-    for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_m[w]);
-    float lt = 0.f;
-    for (int w = 0; w < W; ++w) lt += s_l[w] == 0.f ? 0.f : s_l[w] * expf(s_m[w] - mx);
-    for (int d = threadIdx.x; d < HD; d += SIMPLE_THREADS) {
-        float acc = 0.f;
-        for (int w = 0; w < W; ++w) acc += s_l[w] == 0.f ? 0.f : s_o[w][d] * expf(s_m[w] - mx);
-        out[((size_t)(sq.off + i) * H + h) * HD + d] = from_f32<T>(acc / lt);
-    }
-}
-
 // The step kernel serves every sequence of at most STEP_MAX_ROWS query rows
 // per KV head; it is left out when the host's sizes say that there is none.
 bool uses_step(const KvbBatch& b, int G) {
@@ -635,6 +546,7 @@ int at_kvb_attention(at_ctx* ctx, const at_kvb* cache, const at_token_batch* bat
         AT_REQUIRE(dtype == AT_GGML_F32 || dtype == AT_GGML_F16 || dtype == AT_GGML_BF16, AT_ERR_UNSUPPORTED,
                    "query type must be F32, F16 or BF16");
         AT_REQUIRE(n_heads > 0 && n_heads % c.hkv == 0, AT_ERR_INVALID_ARG, "query heads must be a multiple of the KV heads");
+        AT_REQUIRE(n_heads / c.hkv <= 128, AT_ERR_UNSUPPORTED, "at most 128 query heads per KV head");
         AT_REQUIRE(window >= 0, AT_ERR_INVALID_ARG, "window must not be negative");
         AT_REQUIRE(scale > 0.f && scale < INFINITY, AT_ERR_INVALID_ARG, "scale must be positive and finite");
         if (b.n_seqs == 0 || b.max_tokens == 0) return;
@@ -655,16 +567,8 @@ int at_kvb_attention(at_ctx* ctx, const at_kvb* cache, const at_token_batch* bat
                 else launch_step<T, 64>(p, s, ctx->stream);
             });
         }
-        if (b.max_tokens * (n_heads / c.hkv) <= STEP_MAX_ROWS) return;
-        const int64_t grid = (int64_t)b.n_seqs * b.max_tokens * n_heads;
-        AT_REQUIRE(grid <= INT32_MAX, AT_ERR_INVALID_ARG, "the batch is too large for one call");
-        kvb_dispatch(dtype, [&](auto t) {
-            using T = decltype(t);
-            auto kern = c.hd == 128 ? kvb_attn_simple_kernel<T, 128> : kvb_attn_simple_kernel<T, 64>;
-            kern<<<(int)grid, SIMPLE_THREADS, 0, ctx->stream>>>(c, b, static_cast<const T*>(q), q_token_stride, q_head_stride,
-                                                                static_cast<T*>(out), n_heads, scale, window, STEP_MAX_ROWS);
-        });
-        AT_CUDA(cudaGetLastError());
+        if (b.max_tokens * (n_heads / c.hkv) > STEP_MAX_ROWS)
+            launch_kvb_attn_prompt(c, b, dtype, n_heads, q, q_token_stride, q_head_stride, out, scale, window, STEP_MAX_ROWS, ctx->stream);
     });
 }
 

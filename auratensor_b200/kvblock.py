@@ -272,4 +272,5 @@ class BlockKvCache:
             self.status.zero_()
             raise IllegalStateException(_lib.AT_ERR_STATE, "block KV cache: " + " and ".join(
                 m for b, m in ((_lib.KVB_BAD_SEQ, "a slot, start or offset out of range (its sequence was skipped)"),
+                               (_lib.KVB_STALLED, "a wait inside a kernel that ran out (its output is not valid)"),
                                (_lib.KVB_BAD_BLOCK, "a page outside the pool (writes dropped, reads NaN)")) if bits & b))

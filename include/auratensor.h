@@ -388,6 +388,7 @@ typedef struct at_kvb {
 } at_kvb;
 #define AT_KVB_BAD_SEQ   1         /* slot, start or offset out of range: that sequence was skipped */
 #define AT_KVB_BAD_BLOCK 2         /* block_table entry outside the pool: writes dropped, reads NaN */
+#define AT_KVB_STALLED   4         /* a bounded wait inside a kernel ran out: its output is not valid */
 /* Runs of consecutive tokens, one per sequence, packed one after the other:
  * sequence s has slot slots[s] and the tokens offsets[s] .. offsets[s+1] of the
  * packed arrays, at positions starts[s], starts[s] + 1, ... The arrays are on
