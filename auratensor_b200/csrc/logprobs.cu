@@ -7,6 +7,18 @@
 // Rows without a distribution: all -inf gives lse -inf, log p -inf, H 0;
 // a NaN or +inf gives NaN for lse, log p and H. The alternatives are ordered
 // all the same, NaN above +inf.
+//
+// One pass over the logits, which is what bounds it: each thread keeps its own
+// running maximum and sums (FP32, joined at the end), 64 bytes of a row per
+// thread and step in flight. The alternatives ride along: a bound tau, which
+// at least k logits of the row reach, is found from the maxima of groups of
+// lanes in the first step (and again whenever many threads exceed it); what is
+// above tau, a few times k values, goes to a shared-memory list that is ranked
+// at the end, and if fewer than k are above, the first ids equal to tau fill
+// up. A row is one CTA, or a cluster of up to 8 whose parts meet in distributed
+// shared memory when there are too few rows to fill the GPU.
+#include <cooperative_groups.h>
+
 #include <cstdint>
 #include <string>
 
@@ -16,8 +28,17 @@ namespace at {
 
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int LP_THREADS = 512;
+constexpr int LP_WARPS = LP_THREADS / 32;
 constexpr int LP_TOP_MAX = 32;
+constexpr int LP_VECS = 4;                       // 16-byte vectors per thread and step
+constexpr int LP_GROUP = 8;                      // lanes whose maximum counts as one for tau
+constexpr int LP_GROUPS = LP_THREADS / LP_GROUP; // >= LP_TOP_MAX
+constexpr int LP_LIST = 2048;                    // values above tau
+constexpr int LP_RAISE = 64;                     // threads above tau in one step that make it be found again
+constexpr int LP_MAX_CLUSTER = 8;
 
 // Order-preserving bits: NaN on top, -0 equal to +0.
 __device__ __forceinline__ uint32_t lp_key(float v) {
@@ -25,79 +46,385 @@ __device__ __forceinline__ uint32_t lp_key(float v) {
     const uint32_t u = __float_as_uint(v + 0.f);
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
+// Larger value first, then the lower id.
 __device__ __forceinline__ unsigned long long lp_pack(float v, int i) {
     return ((unsigned long long)lp_key(v) << 32) | (0xFFFFFFFFu - (uint32_t)i);
 }
+__device__ __forceinline__ int lp_id(unsigned long long p) { return (int)(0xFFFFFFFFu - (uint32_t)p); }
 
-template <class R, class F>
-__device__ __forceinline__ R lp_block_reduce(R v, R* s, F f) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ __forceinline__ float lp_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Two FP32 lanes in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(r)) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(r)) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(r))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
+    return r;
+}
+
+// Word w of a 16-byte vector: two 16-bit logits, or one FP32 logit.
+template <class T>
+struct Words;
+template <>
+struct Words<float> {
+    static constexpr uint32_t NINF = 0xFF800000u;  // -inf in every lane of a word
+    static __device__ __forceinline__ float max_of(const uint4* v) {
+        float m = -INFINITY;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if (lane == 0) s[warp] = v;
-    __syncthreads();
-    v = s[0];
-    for (int w = 1; w < LP_THREADS / 32; ++w) v = f(v, s[w]);
-    return v;
+        for (int i = 0; i < LP_VECS; ++i)
+            m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(v[i].x), __uint_as_float(v[i].y)), fmaxf(__uint_as_float(v[i].z), __uint_as_float(v[i].w))));
+        return m;
+    }
+    static __device__ __forceinline__ float2 pair(const uint4& v, int j) {  // j 0..1
+        return j ? make_float2(__uint_as_float(v.z), __uint_as_float(v.w)) : make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+    }
+};
+template <class H2>
+__device__ __forceinline__ float max16(const uint4* v) {
+    const H2* h = reinterpret_cast<const H2*>(v);
+    H2 m = h[0];
+#pragma unroll
+    for (int i = 1; i < 4 * LP_VECS; ++i) m = __hmax2(m, h[i]);
+    return fmaxf((float)m.x, (float)m.y);
+}
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
+template <>
+struct Words<__half> {
+    static constexpr uint32_t NINF = 0xFC00FC00u;
+    static __device__ __forceinline__ float max_of(const uint4* v) { return max16<__half2>(v); }
+    static __device__ __forceinline__ float2 pair(const uint4& v, int j) {
+        const uint32_t w = word_of(v, j);
+        return __half22float2(reinterpret_cast<const __half2&>(w));
+    }
+};
+template <>
+struct Words<__nv_bfloat16> {
+    static constexpr uint32_t NINF = 0xFF80FF80u;
+    static __device__ __forceinline__ float max_of(const uint4* v) { return max16<__nv_bfloat162>(v); }
+    static __device__ __forceinline__ float2 pair(const uint4& v, int j) {
+        const uint32_t w = word_of(v, j);
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    }
+};
+
+// Running maximum and sums of one thread (or of a joined set): s = sum e^(x - m),
+// t = sum (x - m) e^(x - m).
+struct Sums {
+    float m, s, t;
+    __device__ __forceinline__ void move(float to) {  // to >= m
+        const float d = m - to, a = __expf(d);
+        t = a == 0.f ? 0.f : a * fmaf(d, s, t);  // d may be -inf
+        s *= a;                                  // a NaN stays
+        m = to;
+    }
+    __device__ __forceinline__ void join(Sums o) {
+        const float to = fmaxf(m, o.m);
+        if (to != -INFINITY) {  // else no logit has weight in either
+            if (m != to) move(to);
+            if (o.m != to) o.move(to);
+        }
+        s += o.s;
+        t += o.t;
+        m = to;
+    }
+    __device__ __forceinline__ void add(float x) {
+        if (x > m) move(x);
+        const float d = x - (m == -INFINITY ? 0.f : m), e = __expf(d);
+        s += e;
+        t += e == 0.f ? 0.f : e * d;
+    }
+};
+
+struct LpShared {
+    unsigned long long list[LP_LIST];
+    unsigned long long top[LP_TOP_MAX];          // the CTA's k best, in order (0: fewer)
+    unsigned long long best_of_row[LP_TOP_MAX];  // the cluster's
+    unsigned long long best[LP_WARPS];
+    float group[LP_GROUPS];
+    Sums part[LP_WARPS], sums;
+    unsigned count;
+    int eq[LP_WARPS];
+    float tau;
+};
+
+struct LpParams {
+    const void* logits;
+    int64_t stride;
+    int V, k, splits;
+    const int32_t* tokens;
+    float *lp, *lse, *ent;
+    int32_t* ids;
+    float* alt;
+};
+
+// The CTA's k best by rounds of "the largest below the last": for rows with
+// NaN or +inf, and for lists that overflowed.
+template <class T>
+__device__ void lp_top_slow(const T* x, int lo, int hi, int k, LpShared* sh) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    unsigned long long last = ~0ull;
+    for (int j = 0; j < k; ++j) {
+        unsigned long long b = 0;
+        for (int i = lo + tid; i < hi; i += LP_THREADS) {
+            const unsigned long long p = lp_pack(to_f32<T>(x[i]), i);
+            if (p < last && p > b) b = p;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const unsigned long long c = __shfl_xor_sync(0xffffffffu, b, o);
+            b = c > b ? c : b;
+        }
+        __syncthreads();
+        if (lane == 0) sh->best[warp] = b;
+        __syncthreads();
+        for (int w = 0; w < LP_WARPS; ++w) b = sh->best[w] > b ? sh->best[w] : b;
+        last = b;
+        if (tid == 0) sh->top[j] = b;
+        if (b == 0) break;  // fewer than k logits here (the rest of top is 0)
+    }
 }
 
 template <class T>
-__global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const T* __restrict__ logits, int V, int64_t stride,
-                                                              const int32_t* __restrict__ tokens, int k, float* __restrict__ lp,
-                                                              float* __restrict__ lse_out, float* __restrict__ ent,
-                                                              int32_t* __restrict__ ids, float* __restrict__ alt) {
-    __shared__ float s_f[LP_THREADS / 32];
-    __shared__ unsigned long long s_k[LP_THREADS / 32];
-    const T* x = logits + (int64_t)blockIdx.x * stride;
-    unsigned long long best = 0;
-    for (int i = threadIdx.x; i < V; i += LP_THREADS) best = max(best, lp_pack(to_f32<T>(x[i]), i));
-    best = lp_block_reduce(best, s_k, [](unsigned long long a, unsigned long long c) { return a > c ? a : c; });
-    const int top = (int)(0xFFFFFFFFu - (uint32_t)best);
-    const float m = to_f32<T>(x[top]);
-    float s = 0.f, t = 0.f;
-    for (int i = threadIdx.x; i < V; i += LP_THREADS) {
-        const float d = to_f32<T>(x[i]) - m, e = expf(d);
-        s += e;
-        t += e > 0.f ? d * e : 0.f;
+__global__ void __launch_bounds__(LP_THREADS, 3) logprobs_kernel(const LpParams p) {
+    using W = Words<T>;
+    constexpr int VE = 16 / (int)sizeof(T);                 // logits per vector
+    constexpr float L2E = 1.44269504088896341f;
+    __shared__ LpShared sh;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int row = blockIdx.x / p.splits, part = blockIdx.x - row * p.splits;
+    const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.stride;
+    const int k = p.k;
+    // this CTA's ids [lo, hi); vectors of the row start at its first 16-byte boundary
+    const int head = min(p.V, (int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)));
+    const int nv = (p.V - head) / VE;
+    const int v0 = (int)((int64_t)nv * part / p.splits), v1 = (int)((int64_t)nv * (part + 1) / p.splits);
+    const int lo = part == 0 ? 0 : head + v0 * VE, hi = part == p.splits - 1 ? p.V : head + v1 * VE;
+    const uint4* xv = reinterpret_cast<const uint4*>(x + head);
+
+    if (tid == 0) {
+        sh.count = 0;
+        sh.tau = -INFINITY;
     }
-    auto add = [](float a, float c) { return a + c; };
-    s = lp_block_reduce(s, s_f, add);
-    t = lp_block_reduce(t, s_f, add);
+    if (tid < LP_TOP_MAX) sh.top[tid] = 0;
+    __syncthreads();
+    Sums mine{-INFINITY, 0.f, 0.f};
+    // what lies outside the vectors, one logit per thread, listed as it is
+    {
+        const int before = part == 0 ? head : 0, after = part == p.splits - 1 ? p.V - head - nv * VE : 0;
+        const int i = tid < before ? tid : tid - before < after ? head + nv * VE + tid - before : -1;
+        if (i >= 0) {
+            const float v = to_f32<T>(x[i]);
+            mine.add(v);
+            if (k > 0) sh.list[atomicAdd(&sh.count, 1u)] = lp_pack(v, i);
+        }
+    }
+    float tau = -INFINITY;
+    for (int b = v0; b < v1; b += LP_THREADS * LP_VECS) {
+        uint4 v[LP_VECS];
+#pragma unroll
+        for (int i = 0; i < LP_VECS; ++i) {
+            const int at = b + i * LP_THREADS + tid;
+            v[i] = make_uint4(W::NINF, W::NINF, W::NINF, W::NINF);
+            if (at < v1) v[i] = ld_stream_u4(xv + at);
+        }
+        float top = W::max_of(v);
+        if (b + tid < v1) {
+            if (top > mine.m) mine.move(top);
+            const float ref = mine.m == -INFINITY ? 0.f : mine.m;
+            const float2 neg = make_float2(-ref, -ref), l2 = make_float2(L2E, L2E);
+            float2 s = make_float2(0.f, 0.f), t = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < LP_VECS; ++i) {
+                if (b + i * LP_THREADS + tid >= v1) break;
+#pragma unroll
+                for (int j = 0; j < VE / 2; ++j) {
+                    const float2 d = add2(W::pair(v[i], j), neg);
+                    const float2 a = mul2(d, l2), e = make_float2(lp_ex2(a.x), lp_ex2(a.y));
+                    s = add2(s, e);
+                    t = fma2(e, d, t);
+                }
+            }
+            float tt = t.x + t.y;
+            if (tt != tt) {  // -inf logits (0 (-inf)), or NaN, which s shows
+                tt = 0.f;
+#pragma unroll
+                for (int i = 0; i < LP_VECS; ++i)
+#pragma unroll
+                    for (int j = 0; j < VE / 2; ++j) {
+                        const float2 d = add2(W::pair(v[i], j), neg);
+                        const float ex = lp_ex2(d.x * L2E), ey = lp_ex2(d.y * L2E);
+                        tt += (ex == 0.f ? 0.f : ex * d.x) + (ey == 0.f ? 0.f : ey * d.y);
+                    }
+            }
+            mine.s += s.x + s.y;
+            mine.t += tt;
+        }
+        if (k > 0) {
+            const int above = __syncthreads_count(top > tau);
+            if (above > LP_RAISE) {  // uniform
+                float g = top;
+#pragma unroll
+                for (int o = LP_GROUP / 2; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+                if ((tid & (LP_GROUP - 1)) == 0) sh.group[tid / LP_GROUP] = g;
+                __syncthreads();
+                if (tid < LP_GROUPS) {
+                    const float mineg = sh.group[tid];
+                    int rank = 0;
+#pragma unroll 8
+                    for (int j = 0; j < LP_GROUPS; ++j) rank += sh.group[j] > mineg || (sh.group[j] == mineg && j < tid);
+                    if (rank == k - 1) sh.tau = fmaxf(tau, mineg);
+                }
+                __syncthreads();
+                tau = sh.tau;
+            }
+            if (top > tau) {
+#pragma unroll
+                for (int i = 0; i < LP_VECS; ++i)
+#pragma unroll
+                    for (int j = 0; j < VE / 2; ++j) {
+                        const float2 y = W::pair(v[i], j);
+                        const int id = head + (b + i * LP_THREADS + tid) * VE + 2 * j;
+                        if (y.x > tau) {
+                            const unsigned at = atomicAdd(&sh.count, 1u);
+                            if (at < LP_LIST) sh.list[at] = lp_pack(y.x, id);
+                        }
+                        if (y.y > tau) {
+                            const unsigned at = atomicAdd(&sh.count, 1u);
+                            if (at < LP_LIST) sh.list[at] = lp_pack(y.y, id + 1);
+                        }
+                    }
+            }
+        }
+    }
+    // the CTA's sums
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        Sums other{__shfl_xor_sync(0xffffffffu, mine.m, o), __shfl_xor_sync(0xffffffffu, mine.s, o), __shfl_xor_sync(0xffffffffu, mine.t, o)};
+        mine.join(other);
+    }
+    if (lane == 0) sh.part[warp] = mine;
+    __syncthreads();
+    Sums all = sh.part[0];
+    for (int w = 1; w < LP_WARPS; ++w) all.join(sh.part[w]);
+    // its k best
+    if (k > 0) {
+        const unsigned n = sh.count;
+        if (all.s != all.s || n > LP_LIST) {
+            lp_top_slow(x, lo, hi, k, &sh);
+        } else {
+            // above tau: ranked; then the first ids equal to tau
+            unsigned above = 0;
+            for (unsigned base = 0; base < n; base += LP_THREADS) {
+                const unsigned i = base + tid;
+                const unsigned long long mk = i < n ? sh.list[i] : 0;
+                const bool in = i < n && (uint32_t)(mk >> 32) > lp_key(tau);
+                above += __syncthreads_count(in);
+                if (in) {
+                    unsigned rank = 0;
+                    for (unsigned j = 0; j < n; ++j) rank += sh.list[j] > mk;
+                    if (rank < (unsigned)k) sh.top[rank] = mk;
+                }
+            }
+            for (int base = lo, have = (int)above; base < hi && have < k; base += LP_THREADS) {  // uniform
+                const int i = base + tid;
+                const bool eq = i < hi && to_f32<T>(x[i]) == tau;
+                const uint32_t ballot = __ballot_sync(0xffffffffu, eq);
+                if (lane == 0) sh.eq[warp] = __popc(ballot);
+                __syncthreads();
+                int before = have, total = 0;
+                for (int w = 0; w < LP_WARPS; ++w) {
+                    before += w < warp ? sh.eq[w] : 0;
+                    total += sh.eq[w];
+                }
+                const int at = before + __popc(ballot & ((1u << lane) - 1u));
+                if (eq && at < k) sh.top[at] = lp_pack(tau, i);
+                have += total;
+                __syncthreads();
+            }
+        }
+    }
+    __syncthreads();
+    cg::cluster_group cluster = cg::this_cluster();
+    if (p.splits > 1) {
+        if (tid == 0) sh.sums = all;
+        cluster.sync();
+        if (part == 0) {
+            for (int r = 1; r < p.splits; ++r) {
+                const LpShared* o = cluster.map_shared_rank(&sh, r);
+                all.join(o->sums);
+            }
+            const int n = p.splits * k;
+            for (int i = tid; i < n; i += LP_THREADS) sh.list[i] = cluster.map_shared_rank(&sh, i / k)->top[i % k];
+            __syncthreads();
+            for (int i = tid; i < n; i += LP_THREADS) {
+                const unsigned long long mk = sh.list[i];
+                int rank = 0;
+                for (int j = 0; j < n; ++j) rank += sh.list[j] > mk;
+                if (mk != 0 && rank < k) sh.best_of_row[rank] = mk;
+            }
+            __syncthreads();
+        }
+        cluster.sync();  // the other CTAs' shared memory has been read
+        if (part != 0) return;
+    }
     const float nan = __uint_as_float(0x7FC00000u);
-    const float ls = logf(s);
-    float lse = m + ls, h = ls - t / s;
-    if (m == -INFINITY) {
+    const float ls = logf(all.s);
+    float lse = all.m + ls, h = ls - all.t / all.s;
+    if (all.s == 0.f) {  // -inf only
         lse = -INFINITY;
         h = 0.f;
-    } else if (!(m < INFINITY)) {
+    } else if (all.s != all.s) {
         lse = h = nan;
     }
-    auto logp = [&](float v) { return lse != lse ? nan : v == -INFINITY ? v : (v - m) - ls; };
-    if (threadIdx.x == 0) {
-        const int r = blockIdx.x;
-        lse_out[r] = lse;
-        ent[r] = h;
-        if (lp) {
-            const int tok = tokens[r];
-            lp[r] = (unsigned)tok < (unsigned)V ? logp(to_f32<T>(x[tok])) : nan;
+    auto logp = [&](float v) { return lse != lse ? nan : v == -INFINITY ? v : (v - all.m) - ls; };
+    if (tid == 0) {
+        p.lse[row] = lse;
+        p.ent[row] = h;
+        if (p.lp) {
+            const int tok = p.tokens[row];
+            p.lp[row] = (unsigned)tok < (unsigned)p.V ? logp(to_f32<T>(x[tok])) : nan;
         }
     }
-    for (int j = 0; j < k; ++j) {
-        if (j > 0) {
-            unsigned long long nb = 0;
-            for (int i = threadIdx.x; i < V; i += LP_THREADS) {
-                const unsigned long long p = lp_pack(to_f32<T>(x[i]), i);
-                if (p < best) nb = max(nb, p);
-            }
-            best = lp_block_reduce(nb, s_k, [](unsigned long long a, unsigned long long c) { return a > c ? a : c; });
-        }
-        if (threadIdx.x == 0) {
-            const int id = (int)(0xFFFFFFFFu - (uint32_t)best);
-            ids[(int64_t)blockIdx.x * k + j] = id;
-            alt[(int64_t)blockIdx.x * k + j] = logp(to_f32<T>(x[id]));
-        }
+    if (tid < k) {
+        const int id = lp_id(p.splits > 1 ? sh.best_of_row[tid] : sh.top[tid]);
+        p.ids[(int64_t)row * k + tid] = id;
+        p.alt[(int64_t)row * k + tid] = logp(to_f32<T>(x[id]));
     }
+}
+
+template <class T>
+void launch_logprobs(LpParams p, int rows, int num_sms, cudaStream_t s) {
+    // As many CTAs per row as fill the GPU once (three are resident per SM),
+    // each with a step of logits at least.
+    const int step = LP_THREADS * LP_VECS * (16 / (int)sizeof(T));
+    int splits = 1;
+    while (splits < LP_MAX_CLUSTER && (int64_t)rows * splits * 2 <= 3 * num_sms && (p.V + 2 * splits - 1) / (2 * splits) >= step / 2) splits *= 2;
+    p.splits = splits;
+    AT_REQUIRE((int64_t)rows * splits <= INT32_MAX, AT_ERR_INVALID_ARG, "logprobs: too many rows for one call");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(rows * splits);
+    cfg.blockDim = dim3(LP_THREADS);
+    cfg.stream = s;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {(unsigned)splits, 1, 1};
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    AT_CUDA(cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, p));
 }
 
 }  // namespace
@@ -126,10 +453,9 @@ int at_logprobs(at_ctx* ctx, const void* logits, int dtype, int rows, int vocab,
         AT_CUDA(cudaSetDevice(ctx->device));
         kvb_dispatch(dtype, [&](auto t) {
             using T = decltype(t);
-            logprobs_kernel<T><<<rows, LP_THREADS, 0, ctx->stream>>>(static_cast<const T*>(logits), vocab, row_stride, tokens, n_top,
-                                                                     logprob, logsumexp, entropy, top_ids, top_logprobs);
+            launch_logprobs<T>(LpParams{logits, row_stride, vocab, n_top, 1, tokens, logprob, logsumexp, entropy, top_ids, top_logprobs}, rows,
+                               ctx->num_sms, ctx->stream);
         });
-        AT_CUDA(cudaGetLastError());
     });
 }
 
