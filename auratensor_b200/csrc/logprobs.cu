@@ -10,12 +10,16 @@
 //
 // One pass over the logits, which is what bounds it: each thread keeps its own
 // running maximum and sums (FP32, joined at the end), 64 bytes of a row per
-// thread and step in flight. The alternatives ride along: a bound tau, which
-// at least k logits of the row reach, is found from the maxima of groups of
-// lanes in the first step (and again whenever many threads exceed it); what is
-// above tau, a few times k values, goes to a shared-memory list that is ranked
-// at the end, and if fewer than k are above, the first ids equal to tau fill
-// up. A row is one CTA, or a cluster of up to 8 whose parts meet in distributed
+// thread and step in flight. The alternatives ride along: what exceeds a bound
+// tau, which leaves at least k logits of the row at or above it, goes to a
+// shared-memory list (a few times k values) that is ranked at the end. tau is
+// the k-th largest of the running maxima of 64 groups of lanes, found after
+// 1, 2, 4, 8 .. steps with the whole CTA (each halves what passes per step),
+// and between those by any warp that sees many of its lanes above tau, from
+// its own lanes' maxima, so that a row whose large logits come late does not
+// flood the list. Ties: tau is set just below its value, so that the logits
+// equal to it are listed, unless there are many (constant or masked rows);
+// then they are left out and the first ids equal to tau fill up at the end. A row is one CTA, or a cluster of up to 8 whose parts meet in distributed
 // shared memory when there are too few rows to fill the GPU.
 #include <cooperative_groups.h>
 
@@ -37,8 +41,10 @@ constexpr int LP_VECS = 4;                       // 16-byte vectors per thread a
 constexpr int LP_GROUP = 8;                      // lanes whose maximum counts as one for tau
 constexpr int LP_GROUPS = LP_THREADS / LP_GROUP; // >= LP_TOP_MAX
 constexpr int LP_LIST = 2048;                    // values above tau
-constexpr int LP_RAISE = 64;                     // threads above tau in one step that make it be found again
+constexpr int LP_RAISE = 12;                     // lanes of a warp above tau that make the warp raise it
+constexpr int LP_TIES = 16;                      // maxima beyond k at or above a new tau: more are ties, and it is set on, not below, its value
 constexpr int LP_MAX_CLUSTER = 8;
+constexpr uint32_t LP_NINF = 0x007FFFFFu;        // lp_key(-inf)
 
 // Order-preserving bits: NaN on top, -0 equal to +0.
 __device__ __forceinline__ uint32_t lp_key(float v) {
@@ -50,6 +56,9 @@ __device__ __forceinline__ uint32_t lp_key(float v) {
 __device__ __forceinline__ unsigned long long lp_pack(float v, int i) {
     return ((unsigned long long)lp_key(v) << 32) | (0xFFFFFFFFu - (uint32_t)i);
 }
+// The value of a key, and the key just below (-0 is skipped: it is +0's equal).
+__device__ __forceinline__ float lp_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
+__device__ __forceinline__ uint32_t lp_below(uint32_t k) { return k == 0x80000000u ? k - 2u : k - 1u; }
 __device__ __forceinline__ int lp_id(unsigned long long p) { return (int)(0xFFFFFFFFu - (uint32_t)p); }
 
 __device__ __forceinline__ float lp_ex2(float x) {
@@ -82,30 +91,24 @@ struct Words;
 template <>
 struct Words<float> {
     static constexpr uint32_t NINF = 0xFF800000u;  // -inf in every lane of a word
-    static __device__ __forceinline__ float max_of(const uint4* v) {
-        float m = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < LP_VECS; ++i)
-            m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(v[i].x), __uint_as_float(v[i].y)), fmaxf(__uint_as_float(v[i].z), __uint_as_float(v[i].w))));
-        return m;
+    static __device__ __forceinline__ float max_of(const uint4& v) {
+        return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
     }
     static __device__ __forceinline__ float2 pair(const uint4& v, int j) {  // j 0..1
         return j ? make_float2(__uint_as_float(v.z), __uint_as_float(v.w)) : make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
     }
 };
 template <class H2>
-__device__ __forceinline__ float max16(const uint4* v) {
-    const H2* h = reinterpret_cast<const H2*>(v);
-    H2 m = h[0];
-#pragma unroll
-    for (int i = 1; i < 4 * LP_VECS; ++i) m = __hmax2(m, h[i]);
+__device__ __forceinline__ float max16(const uint4& v) {
+    const H2* h = reinterpret_cast<const H2*>(&v);
+    const H2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
     return fmaxf((float)m.x, (float)m.y);
 }
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
 template <>
 struct Words<__half> {
     static constexpr uint32_t NINF = 0xFC00FC00u;
-    static __device__ __forceinline__ float max_of(const uint4* v) { return max16<__half2>(v); }
+    static __device__ __forceinline__ float max_of(const uint4& v) { return max16<__half2>(v); }
     static __device__ __forceinline__ float2 pair(const uint4& v, int j) {
         const uint32_t w = word_of(v, j);
         return __half22float2(reinterpret_cast<const __half2&>(w));
@@ -114,7 +117,7 @@ struct Words<__half> {
 template <>
 struct Words<__nv_bfloat16> {
     static constexpr uint32_t NINF = 0xFF80FF80u;
-    static __device__ __forceinline__ float max_of(const uint4* v) { return max16<__nv_bfloat162>(v); }
+    static __device__ __forceinline__ float max_of(const uint4& v) { return max16<__nv_bfloat162>(v); }
     static __device__ __forceinline__ float2 pair(const uint4& v, int j) {
         const uint32_t w = word_of(v, j);
         return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
@@ -131,15 +134,18 @@ struct Sums {
         s *= a;                                  // a NaN stays
         m = to;
     }
-    __device__ __forceinline__ void join(Sums o) {
-        const float to = fmaxf(m, o.m);
-        if (to != -INFINITY) {  // else no logit has weight in either
-            if (m != to) move(to);
-            if (o.m != to) o.move(to);
+    // The sums of all lanes (of groups of W lanes), in every lane.
+    template <int W>
+    __device__ __forceinline__ void join_lanes() {
+        float to = m;
+#pragma unroll
+        for (int o = W / 2; o > 0; o >>= 1) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, o));
+        if (m != to) move(to);  // to is not -inf then
+#pragma unroll
+        for (int o = W / 2; o > 0; o >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, o);
+            t += __shfl_xor_sync(0xffffffffu, t, o);
         }
-        s += o.s;
-        t += o.t;
-        m = to;
     }
     __device__ __forceinline__ void add(float x) {
         if (x > m) move(x);
@@ -158,13 +164,14 @@ struct LpShared {
     Sums part[LP_WARPS], sums;
     unsigned count;
     int eq[LP_WARPS];
-    float tau;
+    float bound;
+    uint32_t tau;  // a key
 };
 
 struct LpParams {
     const void* logits;
     int64_t stride;
-    int V, k, splits;
+    int V, k, splits, log_splits;
     const int32_t* tokens;
     float *lp, *lse, *ent;
     int32_t* ids;
@@ -205,19 +212,19 @@ __global__ void __launch_bounds__(LP_THREADS, 3) logprobs_kernel(const LpParams 
     constexpr float L2E = 1.44269504088896341f;
     __shared__ LpShared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int row = blockIdx.x / p.splits, part = blockIdx.x - row * p.splits;
+    const int row = blockIdx.x >> p.log_splits, part = blockIdx.x & (p.splits - 1);
     const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.stride;
     const int k = p.k;
     // this CTA's ids [lo, hi); vectors of the row start at its first 16-byte boundary
     const int head = min(p.V, (int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)));
     const int nv = (p.V - head) / VE;
-    const int v0 = (int)((int64_t)nv * part / p.splits), v1 = (int)((int64_t)nv * (part + 1) / p.splits);
+    const int v0 = (int)(((int64_t)nv * part) >> p.log_splits), v1 = (int)(((int64_t)nv * (part + 1)) >> p.log_splits);
     const int lo = part == 0 ? 0 : head + v0 * VE, hi = part == p.splits - 1 ? p.V : head + v1 * VE;
     const uint4* xv = reinterpret_cast<const uint4*>(x + head);
 
     if (tid == 0) {
         sh.count = 0;
-        sh.tau = -INFINITY;
+        sh.tau = LP_NINF;
     }
     if (tid < LP_TOP_MAX) sh.top[tid] = 0;
     __syncthreads();
@@ -232,8 +239,8 @@ __global__ void __launch_bounds__(LP_THREADS, 3) logprobs_kernel(const LpParams 
             if (k > 0) sh.list[atomicAdd(&sh.count, 1u)] = lp_pack(v, i);
         }
     }
-    float tau = -INFINITY;
-    for (int b = v0; b < v1; b += LP_THREADS * LP_VECS) {
+    float bound = -INFINITY;
+    for (int b = v0, step = 0; b < v1; b += LP_THREADS * LP_VECS, ++step) {
         uint4 v[LP_VECS];
 #pragma unroll
         for (int i = 0; i < LP_VECS; ++i) {
@@ -241,8 +248,20 @@ __global__ void __launch_bounds__(LP_THREADS, 3) logprobs_kernel(const LpParams 
             v[i] = make_uint4(W::NINF, W::NINF, W::NINF, W::NINF);
             if (at < v1) v[i] = ld_stream_u4(xv + at);
         }
-        float top = W::max_of(v);
-        if (b + tid < v1) {
+        float vtop[LP_VECS], top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < LP_VECS; ++i) {
+            vtop[i] = W::max_of(v[i]);
+            top = fmaxf(top, vtop[i]);
+        }
+        bool some = b + tid < v1;
+        if (some && top == -INFINITY) {  // all -inf adds nothing (NaN would: it is not in the maximum)
+            uint32_t differs = 0;
+#pragma unroll
+            for (int i = 0; i < LP_VECS; ++i) differs |= (v[i].x ^ W::NINF) | (v[i].y ^ W::NINF) | (v[i].z ^ W::NINF) | (v[i].w ^ W::NINF);
+            some = differs != 0;
+        }
+        if (some) {
             if (top > mine.m) mine.move(top);
             const float ref = mine.m == -INFINITY ? 0.f : mine.m;
             const float2 neg = make_float2(-ref, -ref), l2 = make_float2(L2E, L2E);
@@ -274,26 +293,46 @@ __global__ void __launch_bounds__(LP_THREADS, 3) logprobs_kernel(const LpParams 
             mine.t += tt;
         }
         if (k > 0) {
-            const int above = __syncthreads_count(top > tau);
-            if (above > LP_RAISE) {  // uniform
-                float g = top;
+            if ((step & (step + 1)) == 0 || bound == -INFINITY) {  // steps 0, 1, 3, 7, .. and until there is one: uniform
+                float g = mine.m;
 #pragma unroll
                 for (int o = LP_GROUP / 2; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
                 if ((tid & (LP_GROUP - 1)) == 0) sh.group[tid / LP_GROUP] = g;
                 __syncthreads();
                 if (tid < LP_GROUPS) {
-                    const float mineg = sh.group[tid];
-                    int rank = 0;
+                    const float own = sh.group[tid];
+                    int rank = 0, at_least = 0;
 #pragma unroll 8
-                    for (int j = 0; j < LP_GROUPS; ++j) rank += sh.group[j] > mineg || (sh.group[j] == mineg && j < tid);
-                    if (rank == k - 1) sh.tau = fmaxf(tau, mineg);
+                    for (int j = 0; j < LP_GROUPS; ++j) {
+                        const float o = sh.group[j];
+                        at_least += o >= own;
+                        rank += o > own || (o == own && j < tid);
+                    }
+                    if (rank == k - 1) {
+                        sh.bound = own;
+                        if (own > -INFINITY) atomicMax(&sh.tau, at_least > k + LP_TIES ? lp_key(own) : lp_below(lp_key(own)));
+                    }
                 }
                 __syncthreads();
-                tau = sh.tau;
+                bound = sh.bound;
+            } else if (__popc(__ballot_sync(0xffffffffu, top > lp_value(*reinterpret_cast<volatile uint32_t*>(&sh.tau)))) > LP_RAISE) {
+                int rank = 0;
+#pragma unroll 8
+                for (int j = 0; j < 32; ++j) {
+                    const float o = __shfl_sync(0xffffffffu, top, j);
+                    rank += o > top || (o == top && j < lane);
+                }
+                const uint32_t who = __ballot_sync(0xffffffffu, rank == k - 1);
+                const float c = __shfl_sync(0xffffffffu, top, __ffs(who) - 1);
+                const int at_least = __popc(__ballot_sync(0xffffffffu, top >= c));
+                if (lane == 0 && c > -INFINITY) atomicMax(&sh.tau, at_least > k + LP_TIES ? lp_key(c) : lp_below(lp_key(c)));
+                __syncwarp();
             }
+            const float tau = lp_value(*reinterpret_cast<volatile uint32_t*>(&sh.tau));
             if (top > tau) {
 #pragma unroll
-                for (int i = 0; i < LP_VECS; ++i)
+                for (int i = 0; i < LP_VECS; ++i) {
+                    if (vtop[i] <= tau) continue;
 #pragma unroll
                     for (int j = 0; j < VE / 2; ++j) {
                         const float2 y = W::pair(v[i], j);
@@ -307,41 +346,49 @@ __global__ void __launch_bounds__(LP_THREADS, 3) logprobs_kernel(const LpParams 
                             if (at < LP_LIST) sh.list[at] = lp_pack(y.y, id + 1);
                         }
                     }
+                }
             }
         }
     }
     // the CTA's sums
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        Sums other{__shfl_xor_sync(0xffffffffu, mine.m, o), __shfl_xor_sync(0xffffffffu, mine.s, o), __shfl_xor_sync(0xffffffffu, mine.t, o)};
-        mine.join(other);
-    }
+    mine.join_lanes<32>();
     if (lane == 0) sh.part[warp] = mine;
     __syncthreads();
-    Sums all = sh.part[0];
-    for (int w = 1; w < LP_WARPS; ++w) all.join(sh.part[w]);
+    Sums all = sh.part[lane % LP_WARPS];
+    all.join_lanes<LP_WARPS>();
     // its k best
     if (k > 0) {
         const unsigned n = sh.count;
+        const uint32_t tau = sh.tau;
         if (all.s != all.s || n > LP_LIST) {
             lp_top_slow(x, lo, hi, k, &sh);
         } else {
             // above tau: ranked; then the first ids equal to tau
-            unsigned above = 0;
-            for (unsigned base = 0; base < n; base += LP_THREADS) {
-                const unsigned i = base + tid;
-                const unsigned long long mk = i < n ? sh.list[i] : 0;
-                const bool in = i < n && (uint32_t)(mk >> 32) > lp_key(tau);
-                above += __syncthreads_count(in);
-                if (in) {
-                    unsigned rank = 0;
-                    for (unsigned j = 0; j < n; ++j) rank += sh.list[j] > mk;
-                    if (rank < (unsigned)k) sh.top[rank] = mk;
-                }
+            unsigned long long kept[LP_LIST / LP_THREADS];
+#pragma unroll
+            for (int i = 0; i < LP_LIST / LP_THREADS; ++i) {
+                const unsigned at = i * LP_THREADS + tid;
+                kept[i] = at < n ? sh.list[at] : 0;
+                if ((uint32_t)(kept[i] >> 32) <= tau) kept[i] = 0;  // listed before tau rose
+            }
+            __syncthreads();
+            if (tid == 0) sh.count = 0;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < LP_LIST / LP_THREADS; ++i)
+                if (kept[i] != 0) sh.list[atomicAdd(&sh.count, 1u)] = kept[i];
+            __syncthreads();
+            const unsigned above = sh.count;
+            for (unsigned i = tid; i < above; i += LP_THREADS) {
+                const unsigned long long mk = sh.list[i];
+                unsigned rank = 0;
+#pragma unroll 4
+                for (unsigned j = 0; j < above; ++j) rank += sh.list[j] > mk;
+                if (rank < (unsigned)k) sh.top[rank] = mk;
             }
             for (int base = lo, have = (int)above; base < hi && have < k; base += LP_THREADS) {  // uniform
                 const int i = base + tid;
-                const bool eq = i < hi && to_f32<T>(x[i]) == tau;
+                const bool eq = i < hi && lp_key(to_f32<T>(x[i])) == tau;
                 const uint32_t ballot = __ballot_sync(0xffffffffu, eq);
                 if (lane == 0) sh.eq[warp] = __popc(ballot);
                 __syncthreads();
@@ -351,7 +398,7 @@ __global__ void __launch_bounds__(LP_THREADS, 3) logprobs_kernel(const LpParams 
                     total += sh.eq[w];
                 }
                 const int at = before + __popc(ballot & ((1u << lane) - 1u));
-                if (eq && at < k) sh.top[at] = lp_pack(tau, i);
+                if (eq && at < k) sh.top[at] = lp_pack(lp_value(tau), i);
                 have += total;
                 __syncthreads();
             }
@@ -363,10 +410,8 @@ __global__ void __launch_bounds__(LP_THREADS, 3) logprobs_kernel(const LpParams 
         if (tid == 0) sh.sums = all;
         cluster.sync();
         if (part == 0) {
-            for (int r = 1; r < p.splits; ++r) {
-                const LpShared* o = cluster.map_shared_rank(&sh, r);
-                all.join(o->sums);
-            }
+            all = lane < p.splits ? cluster.map_shared_rank(&sh, lane)->sums : Sums{-INFINITY, 0.f, 0.f};
+            all.join_lanes<32>();
             const int n = p.splits * k;
             for (int i = tid; i < n; i += LP_THREADS) sh.list[i] = cluster.map_shared_rank(&sh, i / k)->top[i % k];
             __syncthreads();
@@ -414,6 +459,7 @@ void launch_logprobs(LpParams p, int rows, int num_sms, cudaStream_t s) {
     int splits = 1;
     while (splits < LP_MAX_CLUSTER && (int64_t)rows * splits * 2 <= 3 * num_sms && (p.V + 2 * splits - 1) / (2 * splits) >= step / 2) splits *= 2;
     p.splits = splits;
+    p.log_splits = splits == 1 ? 0 : splits == 2 ? 1 : splits == 4 ? 2 : 3;
     AT_REQUIRE((int64_t)rows * splits <= INT32_MAX, AT_ERR_INVALID_ARG, "logprobs: too many rows for one call");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(rows * splits);
@@ -453,7 +499,7 @@ int at_logprobs(at_ctx* ctx, const void* logits, int dtype, int rows, int vocab,
         AT_CUDA(cudaSetDevice(ctx->device));
         kvb_dispatch(dtype, [&](auto t) {
             using T = decltype(t);
-            launch_logprobs<T>(LpParams{logits, row_stride, vocab, n_top, 1, tokens, logprob, logsumexp, entropy, top_ids, top_logprobs}, rows,
+            launch_logprobs<T>(LpParams{logits, row_stride, vocab, n_top, 1, 0, tokens, logprob, logsumexp, entropy, top_ids, top_logprobs}, rows,
                                ctx->num_sms, ctx->stream);
         });
     });
