@@ -293,25 +293,30 @@ __global__ void __launch_bounds__(LP_THREADS, 3) logprobs_kernel(const LpParams 
             mine.t += tt;
         }
         if (k > 0) {
-            if ((step & (step + 1)) == 0 || bound == -INFINITY) {  // steps 0, 1, 3, 7, .. and until there is one: uniform
+            if (((step & (step + 1)) == 0 && (step == 0 || b + LP_THREADS * LP_VECS < v1)) || bound == -INFINITY) {  // uniform
                 float g = mine.m;
 #pragma unroll
                 for (int o = LP_GROUP / 2; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
                 if ((tid & (LP_GROUP - 1)) == 0) sh.group[tid / LP_GROUP] = g;
                 __syncthreads();
-                if (tid < LP_GROUPS) {
-                    const float own = sh.group[tid];
-                    int rank = 0, at_least = 0;
-#pragma unroll 8
-                    for (int j = 0; j < LP_GROUPS; ++j) {
-                        const float o = sh.group[j];
-                        at_least += o >= own;
-                        rank += o > own || (o == own && j < tid);
-                    }
-                    if (rank == k - 1) {
-                        sh.bound = own;
-                        if (own > -INFINITY) atomicMax(&sh.tau, at_least > k + LP_TIES ? lp_key(own) : lp_below(lp_key(own)));
-                    }
+                // LP_GROUP threads rank a group together
+                const int grp = tid / LP_GROUP, sub = tid % LP_GROUP;
+                const float own = sh.group[grp];
+                int rank = 0, at_least = 0;
+#pragma unroll
+                for (int j = sub; j < LP_GROUPS; j += LP_GROUP) {
+                    const float o = sh.group[j];
+                    at_least += o >= own;
+                    rank += o > own || (o == own && j < grp);
+                }
+#pragma unroll
+                for (int o = LP_GROUP / 2; o > 0; o >>= 1) {
+                    rank += __shfl_xor_sync(0xffffffffu, rank, o);
+                    at_least += __shfl_xor_sync(0xffffffffu, at_least, o);
+                }
+                if (sub == 0 && rank == k - 1) {
+                    sh.bound = own;
+                    if (own > -INFINITY) atomicMax(&sh.tau, at_least > k + LP_TIES ? lp_key(own) : lp_below(lp_key(own)));
                 }
                 __syncthreads();
                 bound = sh.bound;
@@ -379,12 +384,14 @@ __global__ void __launch_bounds__(LP_THREADS, 3) logprobs_kernel(const LpParams 
                 if (kept[i] != 0) sh.list[atomicAdd(&sh.count, 1u)] = kept[i];
             __syncthreads();
             const unsigned above = sh.count;
-            for (unsigned i = tid; i < above; i += LP_THREADS) {
-                const unsigned long long mk = sh.list[i];
+            for (unsigned base = 0; base < above; base += LP_GROUPS) {  // LP_GROUP threads rank a logit together
+                const unsigned i = base + tid / LP_GROUP;
+                const unsigned long long mk = i < above ? sh.list[i] : 0;
                 unsigned rank = 0;
-#pragma unroll 4
-                for (unsigned j = 0; j < above; ++j) rank += sh.list[j] > mk;
-                if (rank < (unsigned)k) sh.top[rank] = mk;
+                for (unsigned j = tid % LP_GROUP; j < above; j += LP_GROUP) rank += sh.list[j] > mk;
+#pragma unroll
+                for (int o = LP_GROUP / 2; o > 0; o >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+                if (mk != 0 && rank < (unsigned)k) sh.top[rank] = mk;
             }
             for (int base = lo, have = (int)above; base < hi && have < k; base += LP_THREADS) {  // uniform
                 const int i = base + tid;
@@ -415,10 +422,13 @@ __global__ void __launch_bounds__(LP_THREADS, 3) logprobs_kernel(const LpParams 
             const int n = p.splits * k;
             for (int i = tid; i < n; i += LP_THREADS) sh.list[i] = cluster.map_shared_rank(&sh, i / k)->top[i % k];
             __syncthreads();
-            for (int i = tid; i < n; i += LP_THREADS) {
-                const unsigned long long mk = sh.list[i];
+            for (int base = 0; base < n; base += LP_GROUPS) {
+                const int i = base + tid / LP_GROUP;
+                const unsigned long long mk = i < n ? sh.list[i] : 0;
                 int rank = 0;
-                for (int j = 0; j < n; ++j) rank += sh.list[j] > mk;
+                for (int j = tid % LP_GROUP; j < n; j += LP_GROUP) rank += sh.list[j] > mk;
+#pragma unroll
+                for (int o = LP_GROUP / 2; o > 0; o >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
                 if (mk != 0 && rank < k) sh.best_of_row[rank] = mk;
             }
             __syncthreads();
