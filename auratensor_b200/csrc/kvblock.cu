@@ -68,7 +68,6 @@ KvbBatch kvb_batch(const at_kvb* c, const at_token_batch* b) {
 
 namespace {
 
-constexpr int APPEND_THREADS = 256;
 constexpr uint32_t F32_INF = 0x7F800000u;
 
 template <class T>
@@ -88,10 +87,17 @@ __device__ __forceinline__ uint32_t max_bits8(const float* x) {
     return m;
 }
 
+// Eight quants. 1.5 2^23 + x rounds x to the nearest integer (ties to even) in
+// the low bits of the sum: its low byte is q in two's complement (one addition
+// instead of a conversion, which runs at an eighth of its rate).
 __device__ __forceinline__ uint2 quant8(const float* x, float inv) {
-    uint32_t w[2] = {0u, 0u};
+    uint32_t b[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i >> 2] |= ((uint32_t)__float2int_rn(__fmul_rn(x[i], inv)) & 0xFFu) << (8 * (i & 3));
+    for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], inv), 12582912.f));
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        w[i] = __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x0040), __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040), 0x5410);
     return make_uint2(w[0], w[1]);
 }
 
@@ -104,20 +110,18 @@ struct AppendSrc {
 
 // One CTA: one touched block of one sequence and KV head, of K or of V. The
 // block's new rows stay in registers (NCH chunks of 8 values per thread)
-// between the maximum and the quantization, so every value is read once.
-template <class T, int NCH>
-__global__ void __launch_bounds__(APPEND_THREADS) kvb_append_kernel(KvbDev c, KvbBatch b, AppendSrc<T> sk, AppendSrc<T> sv,
-                                                                    int max_touched) {
-    __shared__ uint32_t s_max[APPEND_THREADS / 32];
+// between the maximum and the quantization, so every value is read once; the
+// bound is memory traffic. NT threads: 256 for whole blocks, one warp (no
+// barriers that wait, 16 chunks of one row in half of it) for a few tokens.
+template <class T, int HD, int NT, int NCH>
+__global__ void __launch_bounds__(NT) kvb_append_kernel(KvbDev c, KvbBatch b, AppendSrc<T> sk, AppendSrc<T> sv, int max_touched) {
+    constexpr int CPR = HD / 8;  // chunks per row: a row's chunks are neighbouring lanes
+    __shared__ uint32_t s_max[NT / 32];
     const int tid = threadIdx.x;
-    uint32_t w = blockIdx.x;
-    const bool is_v = w & 1;
-    w >>= 1;
-    const int h = w % c.hkv;
-    w /= c.hkv;
-    const int j = w % max_touched, s = w / max_touched;
+    const bool is_v = blockIdx.y & 1;
+    const int h = blockIdx.y >> 1, s = blockIdx.x / max_touched, j = blockIdx.x - s * max_touched;
     const KvbSeq q = kvb_seq(c, b, s);
-    const int B = 1 << c.lb, hd = c.hd, cpr = hd >> 3;  // chunks per row
+    const int B = 1 << c.lb;
     const int start = (int)q.start, end = start + q.n;
     const int first = start >> c.lb, blk = first + j, base = blk << c.lb;
     if (q.n == 0 || base >= end) return;
@@ -127,10 +131,10 @@ __global__ void __launch_bounds__(APPEND_THREADS) kvb_append_kernel(KvbDev c, Kv
     const T* x0 = src.x + (int64_t)q.off * src.ts + (int64_t)h * src.hs;
     const int lo = max(start, base), hi = min(end, base + B);
     const size_t row0 = ((size_t)page * c.hkv + h) << c.lb;
-    int8_t* dst = (is_v ? c.v : c.k) + row0 * hd;
+    int8_t* dst = (is_v ? c.v : c.k) + row0 * HD;
     float* scale = (is_v ? c.vs : c.ks) + (size_t)page * c.hkv + h;
     const size_t ring0 = ((size_t)q.slot * c.hkv + h) << (c.lb + 1);
-    T* tail = static_cast<T*>(is_v ? c.vt : c.kt) + ring0 * hd;
+    T* tail = static_cast<T*>(is_v ? c.vt : c.kt) + ring0 * HD;
     float* tail_max = (is_v ? c.vtm : c.ktm) + ring0;
     const int last = (end - 1) >> c.lb;
     const int ring_mask = 2 * B - 1;
@@ -142,123 +146,139 @@ __global__ void __launch_bounds__(APPEND_THREADS) kvb_append_kernel(KvbDev c, Kv
     const int clash = (open && last >= first + 2) ? last - ((last - first) & 1) : -1;
     const bool keep = blk >= last - 1 && blk != clash;
 
-    float x[NCH][8];
+    const float held = *scale;  // the scale of the block's older rows
     uint32_t m = 0;
+    for (int r = base + tid; r < lo; r += NT) m = max(m, __float_as_uint(tail_max[r & ring_mask]) & 0x7FFFFFFFu);
+    float x[NCH][8];
+    const int r0 = tid / CPR, col = 8 * (tid % CPR);  // chunk i of this thread: row r0 + i NT / CPR
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-        const int ch = i * APPEND_THREADS + tid, r = ch / cpr, col = (ch - r * cpr) * 8;
-        const int p = base + r;
-        const bool live = p >= lo && p < hi && r < B;
-        uint32_t rm = 0;
-        if (live) {
-            load8<T>(x0 + (int64_t)(p - start) * src.ts + col, src.vec, x[i]);
-            rm = max_bits8(x[i]);
-        }
+        const int p = lo + r0 + i * (NT / CPR);
+        if (p < hi) load8<T>(x0 + (int64_t)(p - start) * src.ts + col, src.vec, x[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        const int p = lo + r0 + i * (NT / CPR);
+        uint32_t rm = p < hi ? max_bits8(x[i]) : 0;
         m = max(m, rm);
-        if (keep) {  // CTA-uniform; a row's chunks are cpr (8 or 16) neighbouring lanes
-            for (int o = cpr >> 1; o > 0; o >>= 1) rm = max(rm, __shfl_xor_sync(0xffffffffu, rm, o));
-            if (live) {
-                store8<T>(tail + (size_t)(p & ring_mask) * hd + col, x[i]);
+        if (keep) {  // CTA-uniform
+#pragma unroll
+            for (int o = CPR >> 1; o > 0; o >>= 1) rm = max(rm, __shfl_xor_sync(0xffffffffu, rm, o));
+            if (p < hi) {
+                store8<T>(tail + (size_t)(p & ring_mask) * HD + col, x[i]);
                 if (col == 0) tail_max[p & ring_mask] = __uint_as_float(rm);
             }
         }
     }
-    if (base + tid < lo) m = max(m, __float_as_uint(tail_max[(base + tid) & ring_mask]) & 0x7FFFFFFFu);
     m = __reduce_max_sync(0xffffffffu, m);
-    if ((tid & 31) == 0) s_max[tid >> 5] = m;
-    const float held = *scale;  // the scale of the block's older rows
-    __syncthreads();
+    if constexpr (NT > 32) {
+        if ((tid & 31) == 0) s_max[tid >> 5] = m;
+        __syncthreads();
 #pragma unroll
-    for (int i = 0; i < APPEND_THREADS / 32; ++i) m = max(m, s_max[i]);
+        for (int i = 0; i < NT / 32; ++i) m = max(m, s_max[i]);
+    }
     float d = __fdiv_rn(__uint_as_float(m), 127.f), inv = 0.f;
-    if (m >= F32_INF) d = __uint_as_float(0x7FC00000u);
+    const bool poison = m >= F32_INF;
+    if (poison) d = __uint_as_float(0x7FC00000u);
     else if (d < 0x1p-126f) d = 0.f;
     else inv = __fdiv_rn(1.f, d);
-    const bool poison = m >= F32_INF;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-        const int ch = i * APPEND_THREADS + tid, r = ch / cpr, col = (ch - r * cpr) * 8;
-        if (base + r >= lo && base + r < hi && r < B)
-            *reinterpret_cast<uint2*>(dst + (size_t)r * hd + col) = poison ? make_uint2(0u, 0u) : quant8(x[i], inv);
+        const int p = lo + r0 + i * (NT / CPR);
+        if (p < hi) *reinterpret_cast<uint2*>(dst + (size_t)(p - base) * HD + col) = poison ? make_uint2(0u, 0u) : quant8(x[i], inv);
     }
     if (__float_as_uint(held) != __float_as_uint(d)) {
-        for (int ch = tid; ch < (lo - base) * cpr; ch += APPEND_THREADS) {
-            const int r = ch / cpr, col = (ch - r * cpr) * 8;
+        for (int p = base + r0; p < lo; p += NT / CPR) {
             float y[8];
-            load8<T>(tail + (size_t)((base + r) & ring_mask) * hd + col, true, y);
-            *reinterpret_cast<uint2*>(dst + (size_t)r * hd + col) = poison ? make_uint2(0u, 0u) : quant8(y, inv);
+            load8<T>(tail + (size_t)(p & ring_mask) * HD + col, true, y);
+            *reinterpret_cast<uint2*>(dst + (size_t)(p - base) * HD + col) = poison ? make_uint2(0u, 0u) : quant8(y, inv);
         }
         if (tid == 0) *scale = d;
     }
     if (j == 0 && clash >= 0) {
         __syncthreads();  // every read of the ring rows is done
         const int cb = clash << c.lb, n = min(end, cb + B) - cb;
-        for (int ch = tid; ch < B * cpr; ch += APPEND_THREADS) {  // whole warps: B * cpr is a multiple of 32
-            const int r = ch / cpr, col = (ch - r * cpr) * 8;
+        for (int r = r0; r < B; r += NT / CPR) {  // whole warps: B is a multiple of the rows per pass, or all lanes leave together
             float y[8];
             uint32_t rm = 0;
             if (r < n) {
                 load8<T>(x0 + (int64_t)(cb + r - start) * src.ts + col, src.vec, y);
                 rm = max_bits8(y);
-                store8<T>(tail + (size_t)((cb + r) & ring_mask) * hd + col, y);
+                store8<T>(tail + (size_t)((cb + r) & ring_mask) * HD + col, y);
             }
-            for (int o = cpr >> 1; o > 0; o >>= 1) rm = max(rm, __shfl_xor_sync(0xffffffffu, rm, o));
+#pragma unroll
+            for (int o = CPR >> 1; o > 0; o >>= 1) rm = max(rm, __shfl_xor_sync(0xffffffffu, rm, o));
             if (r < n && col == 0) tail_max[(cb + r) & ring_mask] = __uint_as_float(rm);
         }
     }
 }
 
 constexpr int READ_THREADS = 256;
-constexpr int READ_TOKENS = 32;  // positions per CTA
+constexpr int READ_TOKENS = 64;  // positions per CTA
 
-// Four values per thread and step; a CTA reads READ_TOKENS positions of one
-// KV head, K or V, and writes them token-major.
-template <class T>
+// A CTA reads READ_TOKENS positions of one KV head, K or V, and writes them
+// token-major: 8 values per thread and row, all of its loads in flight at once.
+template <class T, int HD>
 __global__ void __launch_bounds__(READ_THREADS) kvb_read_kernel(KvbDev c, KvbBatch b, T* __restrict__ ok, T* __restrict__ ov,
                                                                 int chunks) {
-    uint32_t w = blockIdx.x;
-    const int h = w % c.hkv;
-    w /= c.hkv;
-    const int ch = w % chunks;
-    w /= chunks;
-    const bool is_v = ok ? (w & 1) : true;
-    const int s = (ok && ov) ? w >> 1 : w;
+    constexpr int CPR = HD / 8, ROWS = READ_THREADS / CPR, U = READ_TOKENS / ROWS;
+    const bool is_v = ok ? (ov ? blockIdx.y & 1 : false) : true;
+    const int h = ok && ov ? blockIdx.y >> 1 : blockIdx.y;
+    const int s = blockIdx.x / chunks, i0 = (blockIdx.x - s * chunks) * READ_TOKENS;
     const KvbSeq q = kvb_seq(c, b, s);
-    const int i0 = ch * READ_TOKENS, n = min(READ_TOKENS, q.n - i0);
+    const int n = min(READ_TOKENS, q.n - i0);
     if (n <= 0) return;
     const int8_t* src = is_v ? c.v : c.k;
     const float* sc = is_v ? c.vs : c.ks;
-    T* out = is_v ? ov : ok;
-    const int per = c.hd >> 2;
-    for (int e = threadIdx.x; e < n * per; e += READ_THREADS) {
-        const int r = e / per, col = (e - r * per) * 4;
-        const int p = (int)q.start + i0 + r;
-        const int page = kvb_page(c, q.slot, p >> c.lb);
-        const size_t ph = (size_t)max(page, 0) * c.hkv + h;
-        const float d = page < 0 ? __uint_as_float(0x7FC00000u) : sc[ph];
-        const uint32_t x = *reinterpret_cast<const uint32_t*>(src + ((ph << c.lb) + (p & ((1 << c.lb) - 1))) * c.hd + col);
-        T* o = out + ((size_t)(q.off + i0 + r) * c.hkv + h) * c.hd + col;
+    T* out = (is_v ? ov : ok) + ((size_t)(q.off + i0) * c.hkv + h) * HD;
+    const int r0 = threadIdx.x / CPR, col = 8 * (threadIdx.x % CPR), mask = (1 << c.lb) - 1;
+    uint2 x[U];
+    float d[U];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = from_f32<T>(__fmul_rn((float)(int8_t)((x >> (8 * i)) & 0xFFu), d));
+    for (int i = 0; i < U; ++i) {
+        const int r = r0 + i * ROWS;
+        x[i] = make_uint2(0u, 0u);
+        d[i] = 0.f;
+        if (r < n) {
+            const int p = (int)q.start + i0 + r;
+            const int page = kvb_page(c, q.slot, p >> c.lb);
+            const size_t ph = (size_t)max(page, 0) * c.hkv + h;
+            d[i] = page < 0 ? __uint_as_float(0x7FC00000u) : sc[ph];
+            x[i] = *reinterpret_cast<const uint2*>(src + ((ph << c.lb) + (p & mask)) * HD + col);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int r = r0 + i * ROWS;
+        if (r >= n) break;
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t w = e < 4 ? x[i].x : x[i].y;
+            y[e] = __fmul_rn(magic_byte(w ^ 0x80808080u, e & 3) - 8388736.f, d[i]);  // 2^23 + 128 + q, exact
+        }
+        store8<T>(out + (size_t)r * c.hkv * HD + col, y);
     }
 }
 
-template <class T>
-void launch_append(const KvbDev& c, const KvbBatch& b, const AppendSrc<T>& k, const AppendSrc<T>& v, int64_t max_end,
-                   cudaStream_t s) {
+template <class T, int HD>
+void launch_append(const KvbDev& c, const KvbBatch& b, const AppendSrc<T>& k, const AppendSrc<T>& v, cudaStream_t s) {
     const int B = 1 << c.lb;
     const int touched = (b.max_tokens + B - 2) / B + 1;
-    const int64_t grid = (int64_t)b.n_seqs * touched * c.hkv * 2;
-    AT_REQUIRE(grid <= INT32_MAX, AT_ERR_INVALID_ARG, "the batch is too large for one append");
-    const int nch = B * c.hd / 8 / APPEND_THREADS;
-    switch (nch) {
-        case 8: kvb_append_kernel<T, 8><<<(int)grid, APPEND_THREADS, 0, s>>>(c, b, k, v, touched); break;
-        case 4: kvb_append_kernel<T, 4><<<(int)grid, APPEND_THREADS, 0, s>>>(c, b, k, v, touched); break;
-        case 2: kvb_append_kernel<T, 2><<<(int)grid, APPEND_THREADS, 0, s>>>(c, b, k, v, touched); break;
-        default: kvb_append_kernel<T, 1><<<(int)grid, APPEND_THREADS, 0, s>>>(c, b, k, v, touched); break;
+    AT_REQUIRE((int64_t)b.n_seqs * touched <= INT32_MAX && c.hkv <= 32767, AT_ERR_INVALID_ARG, "the batch is too large for one append");
+    const dim3 grid(b.n_seqs * touched, 2 * c.hkv);
+    const int few = b.max_tokens * (HD / 8);  // chunks of a sequence's new rows in one block at most
+    if (few <= 32) kvb_append_kernel<T, HD, 32, 1><<<grid, 32, 0, s>>>(c, b, k, v, touched);
+    else if (few <= 128) kvb_append_kernel<T, HD, 32, 4><<<grid, 32, 0, s>>>(c, b, k, v, touched);
+    else {
+        switch (B * HD / 8 / 256) {
+            case 8: kvb_append_kernel<T, HD, 256, 8><<<grid, 256, 0, s>>>(c, b, k, v, touched); break;
+            case 4: kvb_append_kernel<T, HD, 256, 4><<<grid, 256, 0, s>>>(c, b, k, v, touched); break;
+            case 2: kvb_append_kernel<T, HD, 256, 2><<<grid, 256, 0, s>>>(c, b, k, v, touched); break;
+            default: kvb_append_kernel<T, HD, 256, 1><<<grid, 256, 0, s>>>(c, b, k, v, touched); break;
+        }
     }
     AT_CUDA(cudaGetLastError());
-    (void)max_end;
 }
 
 template <class T>
@@ -286,8 +306,9 @@ int at_kvb_append(at_ctx* ctx, const at_kvb* cache, const at_token_batch* batch,
         AT_CUDA(cudaSetDevice(ctx->device));
         kvb_dispatch(cache->dtype, [&](auto t) {
             using T = decltype(t);
-            launch_append<T>(c, b, append_src<T>(k, k_token_stride, k_head_stride),
-                             append_src<T>(v, v_token_stride, v_head_stride), batch->max_end, ctx->stream);
+            const AppendSrc<T> sk = append_src<T>(k, k_token_stride, k_head_stride), sv = append_src<T>(v, v_token_stride, v_head_stride);
+            if (c.hd == 128) launch_append<T, 128>(c, b, sk, sv, ctx->stream);
+            else launch_append<T, 64>(c, b, sk, sv, ctx->stream);
         });
     });
 }
@@ -302,12 +323,13 @@ int at_kvb_read(at_ctx* ctx, const at_kvb* cache, const at_token_batch* batch, i
         AT_REQUIRE(k_out || v_out, AT_ERR_INVALID_ARG, "null outputs");
         AT_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, AT_ERR_INVALID_ARG, "outputs must be 16-byte aligned");
         const int chunks = (b.max_tokens + READ_TOKENS - 1) / READ_TOKENS;
-        const int64_t grid = (int64_t)b.n_seqs * (k_out && v_out ? 2 : 1) * chunks * c.hkv;
-        AT_REQUIRE(grid <= INT32_MAX, AT_ERR_INVALID_ARG, "the batch is too large for one read");
+        AT_REQUIRE((int64_t)b.n_seqs * chunks <= INT32_MAX && c.hkv <= 32767, AT_ERR_INVALID_ARG, "the batch is too large for one read");
+        const dim3 grid(b.n_seqs * chunks, c.hkv * (k_out && v_out ? 2 : 1));
         AT_CUDA(cudaSetDevice(ctx->device));
         kvb_dispatch(out_type, [&](auto t) {
             using T = decltype(t);
-            kvb_read_kernel<T><<<(int)grid, READ_THREADS, 0, ctx->stream>>>(c, b, static_cast<T*>(k_out), static_cast<T*>(v_out), chunks);
+            auto kern = c.hd == 128 ? kvb_read_kernel<T, 128> : kvb_read_kernel<T, 64>;
+            kern<<<grid, READ_THREADS, 0, ctx->stream>>>(c, b, static_cast<T*>(k_out), static_cast<T*>(v_out), chunks);
         });
         AT_CUDA(cudaGetLastError());
     });
