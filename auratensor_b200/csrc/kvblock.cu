@@ -71,12 +71,16 @@ namespace {
 constexpr uint32_t F32_INF = 0x7F800000u;
 
 template <class T>
+__device__ __forceinline__ void store_raw8(T* __restrict__ p, const Raw8<T>& x) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(x.t)[i];
+}
+template <class T>
 __device__ __forceinline__ void store8(T* __restrict__ p, const float* x) {
-    alignas(16) T t[8];
+    Raw8<T> t;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = from_f32<T>(x[i]);
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(t)[i];
+    for (int i = 0; i < 8; ++i) t.t[i] = from_f32<T>(x[i]);
+    store_raw8<T>(p, t);
 }
 
 // Bits of the largest |x| (as unsigned: finite < infinity < NaN).
@@ -125,14 +129,23 @@ __global__ void __launch_bounds__(NT) kvb_append_kernel(KvbDev c, KvbBatch b, Ap
     const int start = (int)q.start, end = start + q.n;
     const int first = start >> c.lb, blk = first + j, base = blk << c.lb;
     if (q.n == 0 || base >= end) return;
-    const int page = kvb_page(c, q.slot, blk);
-    if (page < 0) return;
     const AppendSrc<T> src = is_v ? sv : sk;
     const T* x0 = src.x + (int64_t)q.off * src.ts + (int64_t)h * src.hs;
     const int lo = max(start, base), hi = min(end, base + B);
+    // the source's rows first: they do not wait for the page
+    Raw8<T> x[NCH];
+    const int r0 = tid / CPR, col = 8 * (tid % CPR);  // chunk i of this thread: row r0 + i NT / CPR
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        const int p = lo + r0 + i * (NT / CPR);
+        if (p < hi) load_raw8<T>(x0 + (int64_t)(p - start) * src.ts + col, src.vec, x[i]);
+    }
+    const int page = kvb_page(c, q.slot, blk);
+    if (page < 0) return;
     const size_t row0 = ((size_t)page * c.hkv + h) << c.lb;
     int8_t* dst = (is_v ? c.v : c.k) + row0 * HD;
     float* scale = (is_v ? c.vs : c.ks) + (size_t)page * c.hkv + h;
+    const float held = *scale;  // the scale of the block's older rows
     const size_t ring0 = ((size_t)q.slot * c.hkv + h) << (c.lb + 1);
     T* tail = static_cast<T*>(is_v ? c.vt : c.kt) + ring0 * HD;
     float* tail_max = (is_v ? c.vtm : c.ktm) + ring0;
@@ -146,26 +159,23 @@ __global__ void __launch_bounds__(NT) kvb_append_kernel(KvbDev c, KvbBatch b, Ap
     const int clash = (open && last >= first + 2) ? last - ((last - first) & 1) : -1;
     const bool keep = blk >= last - 1 && blk != clash;
 
-    const float held = *scale;  // the scale of the block's older rows
     uint32_t m = 0;
     for (int r = base + tid; r < lo; r += NT) m = max(m, __float_as_uint(tail_max[r & ring_mask]) & 0x7FFFFFFFu);
-    float x[NCH][8];
-    const int r0 = tid / CPR, col = 8 * (tid % CPR);  // chunk i of this thread: row r0 + i NT / CPR
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         const int p = lo + r0 + i * (NT / CPR);
-        if (p < hi) load8<T>(x0 + (int64_t)(p - start) * src.ts + col, src.vec, x[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-        const int p = lo + r0 + i * (NT / CPR);
-        uint32_t rm = p < hi ? max_bits8(x[i]) : 0;
+        float f[8];
+        uint32_t rm = 0;
+        if (p < hi) {
+            to_f32x8<T>(x[i], f);
+            rm = max_bits8(f);
+        }
         m = max(m, rm);
         if (keep) {  // CTA-uniform
 #pragma unroll
             for (int o = CPR >> 1; o > 0; o >>= 1) rm = max(rm, __shfl_xor_sync(0xffffffffu, rm, o));
             if (p < hi) {
-                store8<T>(tail + (size_t)(p & ring_mask) * HD + col, x[i]);
+                store_raw8<T>(tail + (size_t)(p & ring_mask) * HD + col, x[i]);
                 if (col == 0) tail_max[p & ring_mask] = __uint_as_float(rm);
             }
         }
@@ -185,7 +195,11 @@ __global__ void __launch_bounds__(NT) kvb_append_kernel(KvbDev c, KvbBatch b, Ap
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         const int p = lo + r0 + i * (NT / CPR);
-        if (p < hi) *reinterpret_cast<uint2*>(dst + (size_t)(p - base) * HD + col) = poison ? make_uint2(0u, 0u) : quant8(x[i], inv);
+        if (p < hi) {
+            float f[8];
+            to_f32x8<T>(x[i], f);
+            *reinterpret_cast<uint2*>(dst + (size_t)(p - base) * HD + col) = poison ? make_uint2(0u, 0u) : quant8(f, inv);
+        }
     }
     if (__float_as_uint(held) != __float_as_uint(d)) {
         for (int p = base + r0; p < lo; p += NT / CPR) {
@@ -199,12 +213,14 @@ __global__ void __launch_bounds__(NT) kvb_append_kernel(KvbDev c, KvbBatch b, Ap
         __syncthreads();  // every read of the ring rows is done
         const int cb = clash << c.lb, n = min(end, cb + B) - cb;
         for (int r = r0; r < B; r += NT / CPR) {  // whole warps: B is a multiple of the rows per pass, or all lanes leave together
-            float y[8];
             uint32_t rm = 0;
             if (r < n) {
-                load8<T>(x0 + (int64_t)(cb + r - start) * src.ts + col, src.vec, y);
-                rm = max_bits8(y);
-                store8<T>(tail + (size_t)((cb + r) & ring_mask) * HD + col, y);
+                Raw8<T> y;
+                float f[8];
+                load_raw8<T>(x0 + (int64_t)(cb + r - start) * src.ts + col, src.vec, y);
+                to_f32x8<T>(y, f);
+                rm = max_bits8(f);
+                store_raw8<T>(tail + (size_t)((cb + r) & ring_mask) * HD + col, y);
             }
 #pragma unroll
             for (int o = CPR >> 1; o > 0; o >>= 1) rm = max(rm, __shfl_xor_sync(0xffffffffu, rm, o));

@@ -101,19 +101,32 @@ inline void kvb_dispatch(int dtype, F&& f) {
         default: fail(AT_ERR_UNSUPPORTED, "element type must be F32, F16 or BF16, got " + std::to_string(dtype));
     }
 }
-// Eight consecutive elements as FP32; vec: p is 16-byte aligned.
+// Eight consecutive elements as they are; vec: p is 16-byte aligned.
 template <class T>
-__device__ __forceinline__ void load8(const T* __restrict__ p, bool vec, float* x) {
+struct alignas(16) Raw8 {
+    T t[8];
+};
+template <class T>
+__device__ __forceinline__ void load_raw8(const T* __restrict__ p, bool vec, Raw8<T>& x) {
     if (vec) {
-        alignas(16) T t[8];
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(t)[i] = reinterpret_cast<const uint4*>(p)[i];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(t[i]);
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(x.t)[i] = reinterpret_cast<const uint4*>(p)[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(p[i]);
+        for (int i = 0; i < 8; ++i) x.t[i] = p[i];
     }
+}
+template <class T>
+__device__ __forceinline__ void to_f32x8(const Raw8<T>& r, float* x) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(r.t[i]);
+}
+// Eight consecutive elements as FP32.
+template <class T>
+__device__ __forceinline__ void load8(const T* __restrict__ p, bool vec, float* x) {
+    Raw8<T> r;
+    load_raw8<T>(p, vec, r);
+    to_f32x8<T>(r, x);
 }
 
 inline int kvb_elem_bytes(int dtype) { return dtype == AT_GGML_F32 ? 4 : 2; }
