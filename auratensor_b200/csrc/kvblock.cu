@@ -83,12 +83,29 @@ __device__ __forceinline__ void store8(T* __restrict__ p, const float* x) {
     store_raw8<T>(p, t);
 }
 
-// Bits of the largest |x| (as unsigned: finite < infinity < NaN).
-__device__ __forceinline__ uint32_t max_bits8(const float* x) {
-    uint32_t m = 0;
+// The largest |x| as ordered bits (finite < infinity < NaN), two 16-bit lanes
+// at a time for 16-bit types: their magnitudes order like their bits.
+template <class T>
+__device__ __forceinline__ uint32_t max_bits(const Raw8<T>& x, uint32_t m) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(x.t);
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+        for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+    }
     return m;
+}
+// ... as the bits of an FP32 value.
+template <class T>
+__device__ __forceinline__ uint32_t max_bits_f32(uint32_t m) {
+    if constexpr (sizeof(T) == 4) {
+        return m;
+    } else {
+        const unsigned short h = (unsigned short)max(m & 0xFFFFu, m >> 16);
+        return __float_as_uint(to_f32<T>(reinterpret_cast<const T&>(h))) & 0x7FFFFFFFu;
+    }
 }
 
 // Eight quants. 1.5 2^23 + x rounds x to the nearest integer (ties to even) in
@@ -135,10 +152,13 @@ __global__ void __launch_bounds__(NT) kvb_append_kernel(KvbDev c, KvbBatch b, Ap
     // the source's rows first: they do not wait for the page
     Raw8<T> x[NCH];
     const int r0 = tid / CPR, col = 8 * (tid % CPR);  // chunk i of this thread: row r0 + i NT / CPR
+    const int rows = hi - lo - r0;                    // chunk i exists when i NT / CPR < rows
+    {
+        const T* xp = x0 + (int64_t)(lo - start + r0) * src.ts + col;
+        const int64_t step = src.ts * (NT / CPR);
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-        const int p = lo + r0 + i * (NT / CPR);
-        if (p < hi) load_raw8<T>(x0 + (int64_t)(p - start) * src.ts + col, src.vec, x[i]);
+        for (int i = 0; i < NCH; ++i, xp += step)
+            if (i * (NT / CPR) < rows) load_raw8<T>(xp, src.vec, x[i]);
     }
     const int page = kvb_page(c, q.slot, blk);
     if (page < 0) return;
@@ -159,24 +179,23 @@ __global__ void __launch_bounds__(NT) kvb_append_kernel(KvbDev c, KvbBatch b, Ap
     const int clash = (open && last >= first + 2) ? last - ((last - first) & 1) : -1;
     const bool keep = blk >= last - 1 && blk != clash;
 
-    uint32_t m = 0;
-    for (int r = base + tid; r < lo; r += NT) m = max(m, __float_as_uint(tail_max[r & ring_mask]) & 0x7FFFFFFFu);
+    uint32_t m16 = 0;
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-        const int p = lo + r0 + i * (NT / CPR);
-        float f[8];
-        uint32_t rm = 0;
-        if (p < hi) {
-            to_f32x8<T>(x[i], f);
-            rm = max_bits8(f);
-        }
-        m = max(m, rm);
-        if (keep) {  // CTA-uniform
+    for (int i = 0; i < NCH; ++i)
+        if (i * (NT / CPR) < rows) m16 = max_bits<T>(x[i], m16);
+    uint32_t m = max_bits_f32<T>(m16);
+    for (int r = base + tid; r < lo; r += NT) m = max(m, __float_as_uint(tail_max[r & ring_mask]) & 0x7FFFFFFFu);
+    if (keep) {  // CTA-uniform
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const bool live = i * (NT / CPR) < rows;
+            const int p = (lo + r0 + i * (NT / CPR)) & ring_mask;
+            uint32_t rm = live ? max_bits_f32<T>(max_bits<T>(x[i], 0u)) : 0u;
 #pragma unroll
             for (int o = CPR >> 1; o > 0; o >>= 1) rm = max(rm, __shfl_xor_sync(0xffffffffu, rm, o));
-            if (p < hi) {
-                store_raw8<T>(tail + (size_t)(p & ring_mask) * HD + col, x[i]);
-                if (col == 0) tail_max[p & ring_mask] = __uint_as_float(rm);
+            if (live) {
+                store_raw8<T>(tail + (size_t)p * HD + col, x[i]);
+                if (col == 0) tail_max[p] = __uint_as_float(rm);
             }
         }
     }
@@ -192,15 +211,14 @@ __global__ void __launch_bounds__(NT) kvb_append_kernel(KvbDev c, KvbBatch b, Ap
     if (poison) d = __uint_as_float(0x7FC00000u);
     else if (d < 0x1p-126f) d = 0.f;
     else inv = __fdiv_rn(1.f, d);
+    int8_t* dp = dst + (lo - base + r0) * HD + col;
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-        const int p = lo + r0 + i * (NT / CPR);
-        if (p < hi) {
+    for (int i = 0; i < NCH; ++i)
+        if (i * (NT / CPR) < rows) {
             float f[8];
             to_f32x8<T>(x[i], f);
-            *reinterpret_cast<uint2*>(dst + (size_t)(p - base) * HD + col) = poison ? make_uint2(0u, 0u) : quant8(f, inv);
+            *reinterpret_cast<uint2*>(dp + i * (NT / CPR) * HD) = poison ? make_uint2(0u, 0u) : quant8(f, inv);
         }
-    }
     if (__float_as_uint(held) != __float_as_uint(d)) {
         for (int p = base + r0; p < lo; p += NT / CPR) {
             float y[8];
@@ -216,10 +234,8 @@ __global__ void __launch_bounds__(NT) kvb_append_kernel(KvbDev c, KvbBatch b, Ap
             uint32_t rm = 0;
             if (r < n) {
                 Raw8<T> y;
-                float f[8];
                 load_raw8<T>(x0 + (int64_t)(cb + r - start) * src.ts + col, src.vec, y);
-                to_f32x8<T>(y, f);
-                rm = max_bits8(f);
+                rm = max_bits_f32<T>(max_bits<T>(y, 0u));
                 store_raw8<T>(tail + (size_t)((cb + r) & ring_mask) * HD + col, y);
             }
 #pragma unroll
