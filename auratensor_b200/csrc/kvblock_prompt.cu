@@ -5,14 +5,17 @@
 // tokens of consecutive query blocks times the G heads of the KV head, so
 // every K and V byte is read and converted once for all of them. The keys
 // are walked in tiles of 128:
-//   warps 8..11 (producers) bring a tile's int8 K and V rows from their pages
-//     into registers, turn them into f16 (exact, |q| <= 127) and store them
-//     into a two-stage ring: K K-major, V MN-major, 128-byte swizzle;
-//   warp 12 (one thread) issues S = Q K^T into TMEM, and O += P V with P read
-//     from TMEM; with two query tiles one's products run under the other's
-//     softmax;
-//   warps 0..3 and 4..7 (one thread per query row) run the online softmax of
-//     their tile: S from TMEM, P back over S's own columns as packed f16.
+//   two warpgroups of producers, one for K and one for V, copy a tile's int8
+//     rows from their pages into shared memory (cp.async, each thread its own
+//     chunks: the next tile's are in flight while this one's are converted),
+//     turn them into f16 (exact, |q| <= 127) and store them into a two-stage
+//     ring: K K-major, V MN-major, 128-byte swizzle;
+//   one thread issues S = Q K^T into TMEM, and O += P V with P read from TMEM;
+//     with two query tiles one's products run under the other's softmax, with
+//     one (FP32) S has two buffers and the next S runs under this softmax;
+//   a warpgroup per query tile (one thread per row) runs the online softmax:
+//     S from TMEM, twice (its maximum, then the weights: 128 values would not
+//     stay in registers), P back over S's own columns as packed f16.
 // Arithmetic, per row, in log2 units: t_j = s_j + log2 d_v(j), P_j = 2^(t_j - r)
 // with a reference r that follows the row's largest t; out = sum P_j v8_j /
 // sum P_j / d_v(j). The values' scale is part of the exponent, so P fills
@@ -23,10 +26,15 @@
 // FP32 queries take two f16 parts of Q and of P (22 bits) and one query tile.
 // Within a group of 4 head dimensions the f16 order is 0, 2, 1, 3 (how bytes
 // unpack); Q is stored alike and the output is put back in order.
+// The loops are kept short on purpose (unrolled over 32 columns or one chunk,
+// not over a tile): the roles together run far apart in the code, and with
+// tiles unrolled the instruction cache did not hold them (2 prompts up to 4096
+// tokens: 505 us, the MMA warp at 130 cycles per instruction).
 // Every wait is bounded: one that runs out sets the status bit, and all roles
 // leave.
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "kvblock.cuh"
 #include "kvblock_attn.cuh"
@@ -37,18 +45,21 @@ namespace {
 
 constexpr int PR_KT = 128;             // keys per tile
 constexpr int PR_ROWS = 128;           // query rows per tile
-constexpr int PR_PRODUCERS = 128;
+constexpr int PR_PRODUCERS = 128;      // for K, and as many for V
 constexpr uint32_t PR_TMEM_COLS = 512;
 constexpr int kPrSpinLimit = 1 << 20;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
+// s_full and p_full are per query tile, or per S buffer when there is one tile.
+// The scales' ring is four deep: tile k + 4 is written once S of tile k + 2 is
+// done, which was issued after the softmax of tile k.
 struct PrShared {
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t q_full, s_full[2], p_full[2], o_done;
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], sc_full[4];
+    uint64_t q_full, s_full[2], p_full[2], pv_done, o_done;
     uint32_t tmem;
     int bad;
-    float dk[2][8], lv[2][8], iv[2][8], mv[2][8];  // per stage and 16 keys: d_k, log2 part and reciprocal of d_v, mantissa
+    float dk[4][8], lv[4][8], iv[4][8], mv[4][8];  // per 16 keys: d_k, log2 part and reciprocal of d_v, mantissa
 };
 
 __device__ __forceinline__ void bar_init(uint64_t* bar, uint32_t count) {
@@ -74,11 +85,23 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, PrShare
     return false;
 }
 
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+// The MMA warp runs as a whole, with operands that the compiler knows to be
+// the same in every lane (tile addresses are constants of the block, TMEM
+// addresses literals): they then live in uniform registers, where the
+// instruction wants them. From general registers an MMA took 110 to 150 cycles
+// to issue, twice its 64 on the tensor cores. Only the leader's executes.
+__device__ __forceinline__ void mma_commit(uint64_t* bar, uint32_t leader) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(leader)
+        : "memory");
 }
 // Instruction descriptor of kind::f16: D f32 (bits 4-5 = 1), A and B f16
 // (bits 7-9, 10-12 = 0), B K-major (bit 16 = 0) or MN-major (1), N >> 3 at
@@ -87,23 +110,26 @@ constexpr uint32_t pr_idesc(int m, int n, bool b_mn) {
     return (1u << 4) | (b_mn ? (1u << 16) : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 // Shared-memory descriptors, 128-byte swizzle (layout type 2 at bits 61-63),
-// version 1 (bit 46); addresses and offsets in 16-byte units.
-__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+// version 1 (bit 46); addresses and offsets in 16-byte units: the low word
+// holds the address and the leading offset, the high word the stride. A
+// further byte offset is added to the low word.
+constexpr uint32_t desc_high(uint32_t stride_bytes) { return (stride_bytes >> 4) | (1u << 14) | (2u << 29); }
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lead_units) { return (addr >> 4) | (lead_units << 16); }
+template <uint32_t AHI, uint32_t BHI>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc, uint32_t leader) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "mov.b64 x, {%1, %6};\n\tmov.b64 y, {%2, %7};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(leader), "n"(AHI), "n"(BHI)
+        : "memory");
 }
-__device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) | ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) |
-           (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
-                 "l"(b), "r"(idesc), "r"(acc)
-                 : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
-                 "l"(b), "r"(idesc), "r"(acc)
-                 : "memory");
+template <uint32_t BHI>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc, uint32_t leader) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "mov.b64 y, {%2, %6};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(leader), "n"(BHI)
+        : "memory");
 }
 // 32 consecutive 32-bit columns of this warp's 32 TMEM lanes.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
@@ -144,10 +170,27 @@ constexpr int pr_terms() { return sizeof(T) == 4 ? 2 : 1; }
 template <class T>
 constexpr int pr_tiles() { return sizeof(T) == 4 ? 1 : 2; }  // query tiles per CTA
 template <class T>
-constexpr int pr_threads() { return 128 * pr_tiles<T>() + PR_PRODUCERS + 32; }
+constexpr int pr_threads() { return 128 * pr_tiles<T>() + 2 * PR_PRODUCERS + 128; }
+// Registers per thread of the softmax, producer and MMA warpgroups. Their sums
+// must stay within what the block is launched with (threads x the compiler's
+// bound for that many): a setmaxnreg.inc beyond it would wait for ever.
+template <class T>
+constexpr int pr_softmax_regs() { return pr_tiles<T>() == 2 ? 112 : 208; }
+template <class T>
+constexpr int pr_producer_regs() { return pr_tiles<T>() == 2 ? 96 : 112; }
+template <class T>
+constexpr int pr_mma_regs() { return pr_tiles<T>() == 2 ? 56 : 64; }
+template <class T>
+constexpr int pr_launch_regs() { return 65536 / pr_threads<T>() / 8 * 8; }
+template <class T>
+constexpr bool pr_regs_fit() {
+    return 128 * pr_tiles<T>() * pr_softmax_regs<T>() + 2 * PR_PRODUCERS * pr_producer_regs<T>() + 128 * pr_mma_regs<T>() <=
+           pr_threads<T>() * pr_launch_regs<T>();
+}
+static_assert(pr_regs_fit<float>() && pr_regs_fit<__half>(), "register shares");
 template <class T, int HD>
 constexpr size_t pr_smem() {
-    return (size_t)pr_terms<T>() * pr_tiles<T>() * PR_ROWS * HD * 2 + 2 * (2 * PR_KT * HD * 2) + 1024;
+    return (size_t)pr_terms<T>() * pr_tiles<T>() * PR_ROWS * HD * 2 + 2 * (2 * PR_KT * HD * 2) + 2 * PR_KT * HD;
 }
 
 struct PromptParams {
@@ -168,11 +211,13 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
     constexpr uint32_t TILE = 128 * HD * 2;            // bytes of a Q, K or V tile
     constexpr uint32_t IDESC_S = pr_idesc(PR_ROWS, PR_KT, false), IDESC_O = pr_idesc(PR_ROWS, HD, true);
     constexpr int SM_WARPS = 4 * NQ;
-    extern __shared__ uint8_t pr_raw[];
+    constexpr uint32_t T_O = 256, T_LO = 384;          // TMEM columns: S at 0 and 128, O (per tile), low parts of P (one tile, per buffer)
+    extern __shared__ __align__(1024) uint8_t pr_raw[];
     __shared__ PrShared sh;
-    uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pr_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* qs = pr_raw;
     uint8_t* ks = qs + NQ * TERMS * TILE;
     uint8_t* vs = ks + 2 * TILE;
+    uint8_t* raw = vs + 2 * TILE;                      // int8 of K's and V's next tile
     const KvbDev& c = p.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // late query blocks see the most keys: they go first
@@ -204,12 +249,14 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
             bar_init(&sh.k_full[i], PR_PRODUCERS);
             bar_init(&sh.v_full[i], PR_PRODUCERS);
             bar_init(&sh.k_empty[i], 1);
-            // V's scales are read by the softmax threads until their P is done
             bar_init(&sh.v_empty[i], 1);
+            bar_init(&sh.sc_full[i], 2);
+            bar_init(&sh.sc_full[2 + i], 2);
             bar_init(&sh.s_full[i], 1);
             bar_init(&sh.p_full[i], 128);
         }
         bar_init(&sh.q_full, 128 * NQ);
+        bar_init(&sh.pv_done, 1);
         bar_init(&sh.o_done, 1);
         sh.bad = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -217,13 +264,18 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = sh.tmem;
+    // all 512 columns are this block's, so the allocation begins at 0; the
+    // swizzled tiles need their 1024-byte alignment
+    const bool placed = sh.tmem == 0 && (smem_u32(pr_raw) & 1023) == 0;
+    constexpr uint32_t tmem = 0;
+    if (placed) {
 
     if (warp < SM_WARPS) {
         // ------------------------------------------------------------ softmax
+        regs_inc<pr_softmax_regs<T>()>();
         const int i = warp >> 2, row = tid & 127;
         const uint32_t trow = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-        const uint32_t t_s = trow + 128 * i, t_o = trow + 128 * NQ + 128 * i;
+        const uint32_t t_o = trow + T_O + 128 * i;
         const int tok = t0 + i * QB + row / p.G;
         const bool live = row / p.G < QB && tok < sq.n;
         const int qpos = live ? start + tok : -1;
@@ -267,97 +319,112 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
         float r = -INFINITY, l = 0.f;
         bool ok = true;
         int n = 0;
-        for (int k = lo; k < hi && ok; ++k) {
-            if (k < k_lo[i] || k >= k_hi[i]) continue;
-            const int st = (k - lo) & 1, k0 = k * PR_KT;
-            // the scales come with K
-            ok = bar_wait(&sh.k_full[st], ((k - lo) >> 1) & 1, &sh) && bar_wait(&sh.s_full[i], n & 1, &sh);
+        for (int k = max(lo, k_lo[i]); k < k_hi[i]; ++k, ++n) {
+            const int k0 = k * PR_KT, sc = (k - lo) & 3;
+            const int buf = NQ == 2 ? i : n & 1;       // S buffer and its barriers
+            const uint32_t t_s = trow + 128 * buf;
+            ok = bar_wait(&sh.sc_full[sc], ((k - lo) >> 2) & 1, &sh) && bar_wait(&sh.s_full[buf], (NQ == 2 ? n : n >> 1) & 1, &sh);
             if (!(ok = __all_sync(0xffffffffu, ok))) break;
             fence_after();
-            const bool edge = __any_sync(0xffffffffu, k0 + PR_KT - 1 > qpos || (p.window > 0 && k0 <= qpos - p.window));
-            float mx = -INFINITY;
-            uint32_t sv[32];
+            const float *dk = sh.dk[sc], *lv = sh.lv[sc], *iv = sh.iv[sc], *mv = sh.mv[sc];
+            const int hide_from = min(qpos + 1 - k0, PR_KT);                                // columns at or past it are hidden
+            const int hide_to = p.window > 0 ? max(qpos + 1 - p.window - k0, 0) : 0;       // and those before it
+            const bool edge = __any_sync(0xffffffffu, hide_from < PR_KT || hide_to > 0);
+            auto tile = [&](auto is_edge) {
+                constexpr bool EDGE = decltype(is_edge)::value;
+                uint32_t x[32];
+                float mx = -INFINITY;
 #pragma unroll 1
-            for (int cc = 0; cc < 4; ++cc) {
-                tmem_ld32(t_s + 32 * cc, sv);
-                tmem_ld_wait();
-                if (edge) {
+                for (int cc = 0; cc < 4; ++cc) {
+                    tmem_ld32(t_s + 32 * cc, x);
+                    tmem_ld_wait();
+                    if (EDGE) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const int key = k0 + 32 * cc + e;
-                        if (key > qpos || (p.window > 0 && key <= qpos - p.window)) sv[e] = 0xFF800000u;
+                        for (int e = 0; e < 32; ++e)
+                            if (32 * cc + e >= hide_from || 32 * cc + e < hide_to) x[e] = 0xFF800000u;
+                    }
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        float m[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            m[e] = fmaxf(fmaxf(__uint_as_float(x[16 * hf + e]), __uint_as_float(x[16 * hf + e + 4])),
+                                         fmaxf(__uint_as_float(x[16 * hf + e + 8]), __uint_as_float(x[16 * hf + e + 12])));
+                        const float mm = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+                        const float t = fmaf(mm, dk[2 * cc + hf] * qf, lv[2 * cc + hf]);
+                        mx = fmaxf(mx, EDGE && mm == -INFINITY ? -INFINITY : t);
                     }
                 }
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    float m = __uint_as_float(sv[16 * hf]);
-#pragma unroll
-                    for (int e = 1; e < 16; ++e) m = fmaxf(m, __uint_as_float(sv[16 * hf + e]));
-                    if (m != -INFINITY) mx = fmaxf(mx, fmaf(m, sh.dk[st][2 * cc + hf] * qf, sh.lv[st][2 * cc + hf]));
+                float alpha = 1.f;
+                if (mx > r + 8.f) {
+                    alpha = ex2(r - mx);  // 0 for the first
+                    r = mx;
                 }
-            }
-            float alpha = 1.f;
-            if (mx > r + 8.f) {
-                alpha = ex2(r - mx);  // 0 for the first
-                r = mx;
-            }
-            const float sub = r == -INFINITY ? 0.f : r;
-            float sum = 0.f;
+                const float sub = r == -INFINITY ? 0.f : r;
+                float sum = 0.f;
 #pragma unroll 1
-            for (int cc = 0; cc < 4; ++cc) {
-                uint32_t pk[16], pl[16];
-                tmem_ld32(t_s + 32 * cc, sv);
-                tmem_ld_wait();
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const float f = sh.dk[st][2 * cc + hf] * qf, off = sh.lv[st][2 * cc + hf] - sub, mv = sh.mv[st][2 * cc + hf];
-                    float a0 = 0.f, a1 = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        float x = ex2(fmaf(__uint_as_float(sv[16 * hf + e]), f, off)), y = ex2(fmaf(__uint_as_float(sv[16 * hf + e + 1]), f, off));
-                        const int key = k0 + 32 * cc + 16 * hf + e;
-                        bool hx = false, hy = false;
-                        if (edge) {
-                            hx = key > qpos || (p.window > 0 && key <= qpos - p.window);
-                            hy = key + 1 > qpos || (p.window > 0 && key + 1 <= qpos - p.window);
-                            x = hx ? 0.f : x;
-                            y = hy ? 0.f : y;
-                        }
-                        a0 += x;
-                        a1 += y;
-                        if constexpr (TERMS == 2) {
-                            x = hx ? 0.f : x * mv;
-                            y = hy ? 0.f : y * mv;
-                        }
-                        const uint32_t h = pack_h2(x, y);
-                        pk[8 * hf + e / 2] = h;
-                        if constexpr (TERMS == 2) {
-                            const float2 u = unpack_h2(h);
-                            pl[8 * hf + e / 2] = pack_h2(x - u.x, y - u.y);
-                        }
-                    }
-                    const float a = a0 + a1;
-                    if (a != 0.f) sum = fmaf(a, sh.iv[st][2 * cc + hf], sum);
-                }
-                tmem_st16(t_s + 16 * cc, pk);
-                if constexpr (TERMS == 2) tmem_st16(t_o + 128 + 16 * cc, pl);
-            }
-            l = fmaf(l, alpha, sum);
-            // O of the earlier tiles is complete: its products were issued before this S
-            if (n > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll 1
-                for (int cc = 0; cc < HD / 32; ++cc) {
-                    tmem_ld32(t_o + 32 * cc, sv);
+                for (int cc = 0; cc < 4; ++cc) {
+                    uint32_t pk[16];
+                    [[maybe_unused]] uint32_t pl[16];
+                    tmem_ld32(t_s + 32 * cc, x);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) sv[e] = __float_as_uint(__uint_as_float(sv[e]) * alpha);
-                    tmem_st32(t_o + 32 * cc, sv);
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const float f = dk[2 * cc + hf] * qf, off = lv[2 * cc + hf] - sub;
+                        const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
+                        float2 a = make_float2(0.f, 0.f);
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            const int col = 32 * cc + 16 * hf + e;
+                            const float2 t = fma2(make_float2(__uint_as_float(x[16 * hf + e]), __uint_as_float(x[16 * hf + e + 1])), f2, off2);
+                            float2 w = make_float2(ex2(t.x), ex2(t.y));
+                            const bool h0 = EDGE && (col >= hide_from || col < hide_to), h1 = EDGE && (col + 1 >= hide_from || col + 1 < hide_to);
+                            if (EDGE) w = make_float2(h0 ? 0.f : w.x, h1 ? 0.f : w.y);
+                            a = add2(a, w);
+                            if constexpr (TERMS == 2) {
+                                const float m = mv[2 * cc + hf];
+                                w = make_float2(h0 ? 0.f : w.x * m, h1 ? 0.f : w.y * m);
+                            }
+                            const uint32_t h = pack_h2(w.x, w.y);
+                            pk[8 * hf + e / 2] = h;
+                            if constexpr (TERMS == 2) {
+                                const float2 u = unpack_h2(h);
+                                pl[8 * hf + e / 2] = pack_h2(w.x - u.x, w.y - u.y);
+                            }
+                        }
+                        const float as = a.x + a.y;
+                        sum = EDGE && as == 0.f ? sum : fmaf(as, iv[2 * cc + hf], sum);
+                    }
+                    // P's columns 16 cc .. are S's columns that have been read
+                    tmem_st16(t_s + 16 * cc, pk);
+                    if constexpr (TERMS == 2) tmem_st16(trow + T_LO + 64 * buf + 16 * cc, pl);
                 }
-            }
+                l = fmaf(l, alpha, sum);
+                if (n > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                    // O of the earlier tiles must be complete: with two query
+                    // tiles its product was issued before this S
+                    if (NQ == 1) {
+                        ok = __all_sync(0xffffffffu, bar_wait(&sh.pv_done, (n - 1) & 1, &sh));
+                        fence_after();
+                    }
+                    if (ok) {
+#pragma unroll 1
+                        for (int cc = 0; cc < HD / 32; ++cc) {
+                            tmem_ld32(t_o + 32 * cc, x);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * alpha);
+                            tmem_st32(t_o + 32 * cc, x);
+                        }
+                    }
+                }
+            };
+            if (edge) tile(std::true_type{});
+            else tile(std::false_type{});
+            if (!ok) break;
             tmem_st_wait();
             fence_before();
-            bar_arrive(&sh.p_full[i]);
-            ++n;
+            bar_arrive(&sh.p_full[buf]);
         }
         if (ok && n > 0) ok = bar_wait(&sh.o_done, 0, &sh);
         ok = __all_sync(0xffffffffu, ok);
@@ -385,123 +452,178 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
                 }
             }
         }
-    } else if (warp < SM_WARPS + 4) {
+    } else if (warp < SM_WARPS + 8) {
         // ---------------------------------------------------------- producers
-        constexpr int CPR = HD / 16;                   // 16-byte chunks per row
-        constexpr int CH = PR_KT * CPR / PR_PRODUCERS; // chunks per thread of K, and of V
-        const int pt = tid - 32 * SM_WARPS;
-        const int bmask = (1 << c.lb) - 1;
-        for (int k = lo; k < hi; ++k) {
-            const int st = (k - lo) & 1, use = (k - lo) >> 1, k0 = k * PR_KT;
-            // lanes 0..7: the page and scales of each 16 keys
-            int page = -2;
-            float dk = 0.f, dv = 0.f;
-            if (lane < 8 && k0 + 16 * lane < end) {
-                page = kvb_page(c, sq.slot, (k0 + 16 * lane) >> c.lb);
-                const size_t i = (size_t)max(page, 0) * c.hkv + kvh;
-                dk = page < 0 ? __uint_as_float(0x7FC00000u) : c.ks[i];
-                dv = page < 0 ? __uint_as_float(0x7FC00000u) : c.vs[i];
-            }
-            uint4 x[2][CH];
-#pragma unroll
+        if constexpr (pr_producer_regs<T>() < pr_launch_regs<T>()) regs_dec<pr_producer_regs<T>()>();
+        // Four lanes take 64 bytes of a row, the next four the next row's: in
+        // the swizzled tile their 16-byte stores then fall into distinct banks.
+        constexpr int CH = 4 * NA;                     // 16-byte chunks per thread: rows pt / 4 + 32 j, NA chunks of each
+        const bool is_v = warp >= SM_WARPS + 4;
+        const int pt = tid - 32 * SM_WARPS - (is_v ? PR_PRODUCERS : 0);
+        const int bmask = (1 << c.lb) - 1, r0 = pt >> 2, col = 16 * (pt & 3);
+        const int8_t* src = (is_v ? c.v : c.k) + col;
+        const float* scales = is_v ? c.vs : c.ks;
+        // lanes 0..7: the page of each 16 keys of a tile (-1: outside the pool, -2: past the last key)
+        auto lookup = [&](int k) {
+            const int pos = k * PR_KT + 16 * lane;
+            return lane < 8 && k < hi && pos < end ? kvb_page(c, sq.slot, pos >> c.lb) : -2;
+        };
+        const uint32_t slot = smem_u32(raw) + (is_v ? PR_KT * HD : 0) + 16 * pt;  // chunk i at slot + i * 16 * PR_PRODUCERS
+        auto fetch = [&](int k, int page) {
+            const int k0 = k * PR_KT;
+#pragma unroll 2
             for (int i = 0; i < CH; ++i) {
-                const int ch = i * PR_PRODUCERS + pt, r = ch / CPR, col = 16 * (ch % CPR);
+                const int r = r0 + 32 * (i / NA);
                 const int pg = __shfl_sync(0xffffffffu, page, r >> 4);
-                x[0][i] = x[1][i] = make_uint4(0u, 0u, 0u, 0u);
-                if (k0 + r < end && pg >= 0) {
-                    const size_t at = ((((size_t)pg * c.hkv + kvh) << c.lb) + ((k0 + r) & bmask)) * HD + col;
-                    x[0][i] = ld_stream_u4(c.k + at);
-                    x[1][i] = ld_stream_u4(c.v + at);
+                const bool in = k0 + r < end && pg >= 0;
+                const int8_t* from = src + ((((size_t)max(pg, 0) * c.hkv + kvh) << c.lb) + ((k0 + r) & bmask)) * HD + 64 * (i % NA);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot + i * 16 * PR_PRODUCERS), "l"(from), "r"(in ? 16 : 0) : "memory");
+            }
+            return page == -1 ? __uint_as_float(0x7FC00000u) : page < 0 ? 0.f : scales[(size_t)page * c.hkv + kvh];
+        };
+        auto store = [&](int k, float d) {
+            const int st = (k - lo) & 1, use = (k - lo) >> 1, sc = (k - lo) & 3;
+            if (use > 0 && !__all_sync(0xffffffffu, bar_wait(is_v ? &sh.v_empty[st] : &sh.k_empty[st], (use - 1) & 1, &sh))) return false;
+            if (pt < 32) {
+                if (lane < 8) {
+                    if (is_v) value_scale<TERMS == 2>(d, &sh.lv[sc][lane], &sh.iv[sc][lane], &sh.mv[sc][lane]);
+                    else sh.dk[sc][lane] = d;
+                }
+                __syncwarp();
+                if (lane == 0) bar_arrive(&sh.sc_full[sc]);
+            }
+            uint8_t* dst = (is_v ? vs : ks) + st * TILE;
+#pragma unroll 1
+            for (int i = 0; i < CH; ++i) {
+                const int r = r0 + 32 * (i / NA);
+                const uint4 x = *reinterpret_cast<const uint4*>(raw + (is_v ? PR_KT * HD : 0) + 16 * pt + i * 16 * PR_PRODUCERS);
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    const uint4 y = make_uint4(bytes_h2<false>(w[2 * hf], false), bytes_h2<false>(w[2 * hf], true),
+                                               bytes_h2<false>(w[2 * hf + 1], false), bytes_h2<false>(w[2 * hf + 1], true));
+                    const int cc = (col >> 3) + hf;            // chunk of 8 in atom column i % NA
+                    const uint32_t at = is_v ? (r >> 3) * (NA * 1024) + (i % NA) * 1024 + (r & 7) * 128 + ((cc ^ (r & 7)) << 4)
+                                             : (i % NA) * ATOM_COL + sw128(r, cc);
+                    *reinterpret_cast<uint4*>(dst + at) = y;
                 }
             }
-            if (use > 0 && !(bar_wait(&sh.k_empty[st], (use - 1) & 1, &sh) && bar_wait(&sh.v_empty[st], (use - 1) & 1, &sh))) break;
-            if (pt < 8) {
-                sh.dk[st][pt] = dk;
-                value_scale<TERMS == 2>(dv, &sh.lv[st][pt], &sh.iv[st][pt], &sh.mv[st][pt]);
-            }
-#pragma unroll
-            for (int kv = 0; kv < 2; ++kv) {
-                uint8_t* dst = (kv ? vs : ks) + st * TILE;
-#pragma unroll
-                for (int i = 0; i < CH; ++i) {
-                    const int ch = i * PR_PRODUCERS + pt, r = ch / CPR, c8 = 2 * (ch % CPR);
-                    const uint32_t w[4] = {x[kv][i].x, x[kv][i].y, x[kv][i].z, x[kv][i].w};
-#pragma unroll
-                    for (int hf = 0; hf < 2; ++hf) {
-                        const uint4 y = make_uint4(bytes_h2<false>(w[2 * hf], false), bytes_h2<false>(w[2 * hf], true),
-                                                   bytes_h2<false>(w[2 * hf + 1], false), bytes_h2<false>(w[2 * hf + 1], true));
-                        const int cc = c8 + hf;
-                        const uint32_t at = kv == 0 ? (cc >> 3) * ATOM_COL + sw128(r, cc & 7)
-                                                    : (r >> 3) * (NA * 1024) + (cc >> 3) * 1024 + (r & 7) * 128 + (((cc & 7) ^ (r & 7)) << 4);
-                        *reinterpret_cast<uint4*>(dst + at) = y;
-                    }
-                }
-                fence_async();
-                bar_arrive(kv ? &sh.v_full[st] : &sh.k_full[st]);
-            }
+            fence_async();
+            bar_arrive(is_v ? &sh.v_full[st] : &sh.k_full[st]);
+            return true;
+        };
+        int page = lookup(lo);
+        float d = fetch(lo, page);
+        page = lookup(lo + 1);
+        for (int k = lo; k < hi; ++k) {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            const float d_k = d;
+            if (!store(k, d_k)) break;
+            if (k + 1 < hi) d = fetch(k + 1, page);  // into the slots just read
+            page = lookup(k + 2);
         }
-    } else if (lane == 0) {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else {
+        regs_dec<pr_mma_regs<T>()>();
+        if (warp == SM_WARPS + 8) {
         // ---------------------------------------------------------------- MMA
-        bool ok = bar_wait(&sh.q_full, 0, &sh);
+        const uint32_t leader = lane == 0;
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, bar_wait(bar, parity, &sh)) != 0; };
+        bool ok = wait(&sh.q_full, 0);
         fence_after();
-        auto scores = [&](int i, int st) {
-            const uint32_t ka = smem_u32(ks + st * TILE);
+        auto scores = [&](auto i_, auto buf_, auto st_) {
+            constexpr int i = i_(), buf = buf_(), st = st_();
+            const uint32_t kd = desc_low(smem_u32(pr_raw) + (NQ * TERMS + st) * TILE, 1);
 #pragma unroll
             for (int e = 0; e < TERMS; ++e) {
-                const uint32_t qa = smem_u32(qs + (i * TERMS + e) * TILE);
-#pragma unroll
-                for (int kk = 0; kk < HD / 16; ++kk)
-                    mma_ss(tmem + 128 * i, desc_k_major(qa + (kk >> 2) * ATOM_COL + 32 * (kk & 3)),
-                           desc_k_major(ka + (kk >> 2) * ATOM_COL + 32 * (kk & 3)), IDESC_S, (e > 0 || kk > 0) ? 1u : 0u);
-            }
-            mma_commit(&sh.s_full[i]);
-        };
-        auto values = [&](int i, int st, bool first) {
-            const uint32_t va = smem_u32(vs + st * TILE);
-            const uint32_t o = tmem + 128 * NQ + 128 * i;
-#pragma unroll
-            for (int e = 0; e < TERMS; ++e)
-#pragma unroll
-                for (int kk = 0; kk < PR_KT / 16; ++kk)
-                    mma_ts(o, (e == 0 ? tmem + 128 * i : o + 128) + 8 * kk, desc_mn_major(va + kk * 2 * (NA * 1024), 1024, NA * 1024), IDESC_O,
-                           (!first || e > 0 || kk > 0) ? 1u : 0u);
-        };
-        int n[NQ] = {};
-        for (int k = lo; k <= hi && ok; ++k) {
-            const int st = (k - lo) & 1, pst = st ^ 1;
-            if (k < hi) ok = bar_wait(&sh.k_full[st], ((k - lo) >> 1) & 1, &sh);
-            if (ok && k > lo) ok = bar_wait(&sh.v_full[pst], ((k - 1 - lo) >> 1) & 1, &sh);
-            if (!ok) break;
-            fence_after();
-#pragma unroll
-            for (int i = 0; i < NQ; ++i) {
-                const int q = k - 1;
-                if (q >= max(lo, k_lo[i]) && q < k_hi[i]) {
-                    if (!(ok = bar_wait(&sh.p_full[i], n[i] & 1, &sh))) break;
-                    fence_after();
-                    values(i, pst, n[i] == 0);
-                    ++n[i];
+                const uint32_t qd = desc_low(smem_u32(pr_raw) + (i * TERMS + e) * TILE, 1);
+#pragma unroll 1
+                for (int kk = 0; kk < HD / 16; ++kk) {
+                    const uint32_t off = ((kk >> 2) * ATOM_COL + 32 * (kk & 3)) >> 4;
+                    mma_ss<desc_high(1024), desc_high(1024)>(128 * buf, qd + off, kd + off, IDESC_S, (e > 0 || kk > 0) ? 1u : 0u, leader);
                 }
-                if (k < hi && k >= k_lo[i] && k < k_hi[i]) scores(i, st);
             }
-            if (!ok) break;
-            if (k > lo) mma_commit(&sh.v_empty[pst]);
-            if (k < hi) mma_commit(&sh.k_empty[st]);
+            mma_commit(&sh.s_full[buf], leader);
+        };
+        auto values = [&](auto i_, auto buf_, auto st_, uint32_t acc) {
+            constexpr int i = i_(), buf = buf_(), st = st_();
+            const uint32_t vd = desc_low(smem_u32(pr_raw) + (NQ * TERMS + 2 + st) * TILE, 64);
+#pragma unroll
+            for (int e = 0; e < TERMS; ++e) {
+#pragma unroll 1
+                for (int kk = 0; kk < PR_KT / 16; ++kk)
+                    mma_ts<desc_high(NA * 1024)>(T_O + 128 * i, (e == 0 ? 128 * buf : T_LO + 64 * buf) + 8 * kk, vd + ((kk * 2 * (NA * 1024)) >> 4),
+                                                 IDESC_O, (e > 0 || kk > 0) ? 1u : acc, leader);
+            }
+        };
+        const std::integral_constant<int, 0> c0;
+        const std::integral_constant<int, 1> c1;
+        if constexpr (NQ == 1) {
+            // S of tile k + 1 is issued before P V of tile k
+            for (int k = lo - 1; k < hi && ok; ++k) {
+                const int n = k - lo;
+                if (k + 1 < hi) {
+                    if (!(ok = wait(&sh.k_full[(n + 1) & 1], ((n + 1) >> 1) & 1))) break;
+                    fence_after();
+                    if ((n + 1) & 1) scores(c0, c1, c1);
+                    else scores(c0, c0, c0);
+                    mma_commit(&sh.k_empty[(n + 1) & 1], leader);
+                }
+                if (k < lo) continue;
+                ok = wait(&sh.v_full[n & 1], (n >> 1) & 1) && wait(&sh.p_full[n & 1], (n >> 1) & 1);
+                if (!ok) break;
+                fence_after();
+                if (n & 1) values(c0, c1, c1, 1u);
+                else values(c0, c0, c0, n > 0);
+                mma_commit(&sh.pv_done, leader);
+                mma_commit(&sh.v_empty[n & 1], leader);
+            }
+        } else {
+            int n0 = 0, n1 = 0;
+            // tile k - 1's products with V, then tile k's scores, one query tile after the other
+            auto step = [&](int k, auto st, auto pst) {
+                if (k < hi && !wait(&sh.k_full[st], ((k - lo) >> 1) & 1)) return false;
+                if (k > lo && !wait(&sh.v_full[pst], ((k - 1 - lo) >> 1) & 1)) return false;
+                fence_after();
+                auto query_tile = [&](auto i, int& n) {
+                    if (k > lo && k - 1 >= k_lo[i] && k - 1 < k_hi[i]) {
+                        if (!wait(&sh.p_full[i], n & 1)) return false;
+                        fence_after();
+                        values(i, i, pst, n > 0);
+                        ++n;
+                    }
+                    if (k < hi && k >= k_lo[i] && k < k_hi[i]) scores(i, i, st);
+                    return true;
+                };
+                if (!query_tile(c0, n0) || !query_tile(c1, n1)) return false;
+                if (k > lo) mma_commit(&sh.v_empty[pst], leader);
+                if (k < hi) mma_commit(&sh.k_empty[st], leader);
+                return true;
+            };
+            for (int k = lo; k <= hi && ok; ++k) ok = (k - lo) & 1 ? step(k, c1, c0) : step(k, c0, c1);
         }
-        mma_commit(&sh.o_done);
-        bar_wait(&sh.o_done, 0, &sh);  // nothing in flight when TMEM is freed
+        mma_commit(&sh.o_done, leader);
+        wait(&sh.o_done, 0);  // nothing in flight when TMEM is freed
+        }
     }
+    }  // placed
     fence_before();
     __syncthreads();
-    if (sh.bad && tid == 0) kvb_flag(c.status, KVB_STALLED);
+    if ((sh.bad || !placed) && tid == 0) kvb_flag(c.status, KVB_STALLED);
     if (warp == SM_WARPS)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(PR_TMEM_COLS) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sh.tmem), "r"(PR_TMEM_COLS) : "memory");
 }
 
 template <class T, int HD>
 void prompt_launch(PromptParams p, cudaStream_t s) {
     auto kern = kvb_attn_prompt_kernel<T, HD>;
-    AT_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pr_smem<T, HD>()));
+    static const int regs = [&] {  // per instance
+        AT_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pr_smem<T, HD>()));
+        cudaFuncAttributes a;
+        AT_CUDA(cudaFuncGetAttributes(&a, kern));
+        return a.numRegs;
+    }();
+    AT_REQUIRE(regs == pr_launch_regs<T>(), AT_ERR_CUDA, "prompt attention was built with another register count than its warpgroups share");
     const int per = pr_tiles<T>() * (PR_ROWS / p.G);
     p.blocks = (p.b.max_tokens + per - 1) / per;
     const int64_t grid = (int64_t)p.blocks * p.c.hkv * p.b.n_seqs;
