@@ -469,19 +469,17 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
             return lane < 8 && k < hi && pos < end ? kvb_page(c, sq.slot, pos >> c.lb) : -2;
         };
         const uint32_t slot = smem_u32(raw) + (is_v ? PR_KT * HD : 0) + 16 * pt;  // chunk i at slot + i * 16 * PR_PRODUCERS
-        auto fetch = [&](int k, int page) {
-            const int k0 = k * PR_KT;
-#pragma unroll 2
-            for (int i = 0; i < CH; ++i) {
-                const int r = r0 + 32 * (i / NA);
-                const int pg = __shfl_sync(0xffffffffu, page, r >> 4);
-                const bool in = k0 + r < end && pg >= 0;
-                const int8_t* from = src + ((((size_t)max(pg, 0) * c.hkv + kvh) << c.lb) + ((k0 + r) & bmask)) * HD + 64 * (i % NA);
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot + i * 16 * PR_PRODUCERS), "l"(from), "r"(in ? 16 : 0) : "memory");
-            }
+        auto fetch = [&](int k, int page, int i) {     // chunk i of tile k
+            const int r = r0 + 32 * (i / NA), at = k * PR_KT + r;
+            const int pg = __shfl_sync(0xffffffffu, page, r >> 4);
+            const int8_t* from = src + ((((size_t)max(pg, 0) * c.hkv + kvh) << c.lb) + (at & bmask)) * HD + 64 * (i % NA);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot + i * 16 * PR_PRODUCERS), "l"(from), "r"(at < end && pg >= 0 ? 16 : 0)
+                         : "memory");
+        };
+        auto scale_of = [&](int page) {
             return page == -1 ? __uint_as_float(0x7FC00000u) : page < 0 ? 0.f : scales[(size_t)page * c.hkv + kvh];
         };
-        auto store = [&](int k, float d) {
+        auto store = [&](int k, float d, int next_page) {
             const int st = (k - lo) & 1, use = (k - lo) >> 1, sc = (k - lo) & 3;
             if (use > 0 && !__all_sync(0xffffffffu, bar_wait(is_v ? &sh.v_empty[st] : &sh.k_empty[st], (use - 1) & 1, &sh))) return false;
             if (pt < 32) {
@@ -493,7 +491,7 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
                 if (lane == 0) bar_arrive(&sh.sc_full[sc]);
             }
             uint8_t* dst = (is_v ? vs : ks) + st * TILE;
-#pragma unroll 1
+#pragma unroll 2
             for (int i = 0; i < CH; ++i) {
                 const int r = r0 + 32 * (i / NA);
                 const uint4 x = *reinterpret_cast<const uint4*>(raw + (is_v ? PR_KT * HD : 0) + 16 * pt + i * 16 * PR_PRODUCERS);
@@ -507,20 +505,23 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
                                              : (i % NA) * ATOM_COL + sw128(r, cc);
                     *reinterpret_cast<uint4*>(dst + at) = y;
                 }
+                if (k + 1 < hi) fetch(k + 1, next_page, i);  // into the slot just read
             }
             fence_async();
             bar_arrive(is_v ? &sh.v_full[st] : &sh.k_full[st]);
             return true;
         };
-        int page = lookup(lo);
-        float d = fetch(lo, page);
-        page = lookup(lo + 1);
+        int page = lookup(lo), next = lookup(lo + 1);
+#pragma unroll 1
+        for (int i = 0; i < CH; ++i) fetch(lo, page, i);
+        float d = scale_of(page);
         for (int k = lo; k < hi; ++k) {
+            const float d_next = scale_of(next);
+            const int after = lookup(k + 2);
             asm volatile("cp.async.wait_all;" ::: "memory");
-            const float d_k = d;
-            if (!store(k, d_k)) break;
-            if (k + 1 < hi) d = fetch(k + 1, page);  // into the slots just read
-            page = lookup(k + 2);
+            if (!store(k, d, next)) break;
+            d = d_next;
+            next = after;
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
