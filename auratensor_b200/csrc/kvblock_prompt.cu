@@ -104,10 +104,10 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar, uint32_t leader) {
         : "memory");
 }
 // Instruction descriptor of kind::f16: D f32 (bits 4-5 = 1), A and B f16
-// (bits 7-9, 10-12 = 0), B K-major (bit 16 = 0) or MN-major (1), N >> 3 at
+// (bits 7-9, 10-12 = 0) or both bf16 (1), B K-major (bit 16 = 0) or MN-major (1), N >> 3 at
 // bits 17-22, M >> 4 at bits 24-28.
-constexpr uint32_t pr_idesc(int m, int n, bool b_mn) {
-    return (1u << 4) | (b_mn ? (1u << 16) : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+constexpr uint32_t pr_idesc(int m, int n, bool b_mn, bool bf16) {
+    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? (1u << 16) : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 // Shared-memory descriptors, 128-byte swizzle (layout type 2 at bits 61-63),
 // version 1 (bit 46); addresses and offsets in 16-byte units: the low word
@@ -161,6 +161,14 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Bytes 0 and 2 of w, signed, as bf16 pairs, exactly: 128 + the low seven bits
+// less 128, or 256 when the sign bit is set.
+__device__ __forceinline__ uint32_t bytes_bf2(uint32_t w) {
+    const uint32_t m = (w & 0x007F007Fu) | 0x43004300u, c = (w & 0x00800080u) | 0x43004300u;
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&m), *reinterpret_cast<const __nv_bfloat162*>(&c));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
 // Byte offset of 16-byte chunk c (0..7) of row r in a K-major tile of
 // 64-element (128-byte) rows.
 __device__ __forceinline__ uint32_t sw128(int r, int c) { return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4)); }
@@ -209,7 +217,8 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
     constexpr int NA = HD / 64;                        // 128-byte atom columns of a row
     constexpr uint32_t ATOM_COL = 128 * 128;           // bytes of one atom column of a 128-row K-major tile
     constexpr uint32_t TILE = 128 * HD * 2;            // bytes of a Q, K or V tile
-    constexpr uint32_t IDESC_S = pr_idesc(PR_ROWS, PR_KT, false), IDESC_O = pr_idesc(PR_ROWS, HD, true);
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    constexpr uint32_t IDESC_S = pr_idesc(PR_ROWS, PR_KT, false, BF16), IDESC_O = pr_idesc(PR_ROWS, HD, true, false);
     constexpr int SM_WARPS = 4 * NQ;
     constexpr uint32_t T_O = 256, T_LO = 384;          // TMEM columns: S at 0 and 128, O (per tile), low parts of P (one tile, per buffer)
     extern __shared__ __align__(1024) uint8_t pr_raw[];
@@ -276,43 +285,60 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
         const int i = warp >> 2, row = tid & 127;
         const uint32_t trow = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t t_o = trow + T_O + 128 * i;
-        const int tok = t0 + i * QB + row / p.G;
-        const bool live = row / p.G < QB && tok < sq.n;
+        const int tq = row / p.G, hq = kvh * p.G + row - tq * p.G;  // the row's token of the tile, and its query head
+        const int tok = t0 + i * QB + tq;
+        const bool live = tq < QB && tok < sq.n;
         const int qpos = live ? start + tok : -1;
-        float qf;  // score factor of the row, log2 units
+        float qf = 1.f;  // power of two of the row (FP32 queries), then its score factor, log2 units
         {
-            const T* src = static_cast<const T*>(p.q) + (int64_t)(sq.off + tok) * p.q_ts + (int64_t)(kvh * p.G + row % p.G) * p.q_hs;
-            float top = 0.f;
-            if (live) {
-#pragma unroll 4
-                for (int d = 0; d < HD; d += 8) {
-                    float x[8];
-                    load8<T>(src + d, p.q_vec, x);
+            // HD / 8 lanes take a row together (a thread's own row would touch
+            // 32 lines per load).
+            constexpr int LPR = HD / 8, RPP = 32 / LPR, PASSES = 32 / RPP, IN_FLIGHT = 8 / TERMS;
+            const int sub = lane / LPR, d = 8 * (lane % LPR), r_w = 32 * (warp & 3);
+            const int64_t own = live ? (int64_t)(sq.off + tok) * p.q_ts + (int64_t)hq * p.q_hs : -1;
+            uint8_t* dst = qs + i * TERMS * TILE + (d >> 6) * ATOM_COL;
+#pragma unroll 1
+            for (int b = 0; b < PASSES; b += IN_FLIGHT) {
+                Raw8<T> raw8[IN_FLIGHT];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+                for (int j = 0; j < IN_FLIGHT; ++j) {
+                    const int64_t at = __shfl_sync(0xffffffffu, own, (b + j) * RPP + sub);
+#pragma unroll
+                    for (int e = 0; e < TERMS; ++e) reinterpret_cast<uint4*>(raw8[j].t)[e] = make_uint4(0u, 0u, 0u, 0u);
+                    if (at >= 0) load_raw8<T>(static_cast<const T*>(p.q) + at + d, p.q_vec, raw8[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < IN_FLIGHT; ++j) {
+                    uint8_t* to = dst + sw128(r_w + (b + j) * RPP + sub, (d >> 3) & 7);
+                    if constexpr (TERMS == 1) {
+                        // 16-bit queries go in as they are (BF16 against BF16 K), pairs (0, 2), (1, 3), ..
+                        const uint4 v = *reinterpret_cast<const uint4*>(raw8[j].t);
+                        *reinterpret_cast<uint4*>(to) = make_uint4(__byte_perm(v.x, v.y, 0x5410), __byte_perm(v.x, v.y, 0x7632),
+                                                                   __byte_perm(v.z, v.w, 0x5410), __byte_perm(v.z, v.w, 0x7632));
+                    } else {
+                        float x[8], top = 0.f;
+                        to_f32x8<T>(raw8[j], x);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+#pragma unroll
+                        for (int o = LPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        const float rs = row_scale(top);
+                        const float mine = __shfl_sync(0xffffffffu, rs, (lane % RPP) * LPR);  // of row (b + j) RPP + lane % RPP
+                        if (lane / RPP == b + j) qf = mine;                                    // the row's own thread
+                        uint32_t h[4], l[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float a = x[4 * (e >> 1) + (e & 1)] * rs, c2 = x[4 * (e >> 1) + (e & 1) + 2] * rs;
+                            h[e] = pack_h2(a, c2);
+                            const float2 g = unpack_h2(h[e]);
+                            l[e] = pack_h2(a - g.x, c2 - g.y);
+                        }
+                        *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
+                        *reinterpret_cast<uint4*>(to + TILE) = make_uint4(l[0], l[1], l[2], l[3]);
+                    }
                 }
             }
-            const float rs = row_scale(top);
-            qf = p.scale * 1.44269504088896341f / rs;
-            uint8_t* dst = qs + i * TERMS * TILE;
-#pragma unroll 4
-            for (int d = 0; d < HD; d += 8) {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = 0.f;
-                if (live) load8<T>(src + d, p.q_vec, x);
-                uint32_t h[4], l[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {  // pairs (0, 2), (1, 3), (4, 6), (5, 7)
-                    const float a = x[4 * (e >> 1) + (e & 1)] * rs, b = x[4 * (e >> 1) + (e & 1) + 2] * rs;
-                    h[e] = pack_h2(a, b);
-                    const float2 f = unpack_h2(h[e]);
-                    l[e] = pack_h2(a - f.x, b - f.y);
-                }
-                const uint32_t at = (d >> 6) * ATOM_COL + sw128(row, (d >> 3) & 7);
-                *reinterpret_cast<uint4*>(dst + at) = make_uint4(h[0], h[1], h[2], h[3]);
-                if constexpr (TERMS == 2) *reinterpret_cast<uint4*>(dst + TILE + at) = make_uint4(l[0], l[1], l[2], l[3]);
-            }
+            qf = p.scale * 1.44269504088896341f / qf;
             fence_async();
             bar_arrive(&sh.q_full);
         }
@@ -431,25 +457,37 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
         if (ok && n > 0) {
             fence_after();
             const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
-            T* dst = static_cast<T*>(p.out) + ((size_t)(sq.off + tok) * p.H + kvh * p.G + row % p.G) * HD;
+            // rows go through the query tiles' shared memory (their last product
+            // is done) to leave as whole lines; chunks are XOR-swizzled by row
+            constexpr int PER = 16 / sizeof(T), CPR = HD / PER, LINE = HD * (int)sizeof(T);
+            uint8_t* own_row = qs + i * TERMS * TILE + row * LINE;
 #pragma unroll 1
             for (int cc = 0; cc < HD / 32; ++cc) {
                 uint32_t ov[32];
                 tmem_ld32(t_o + 32 * cc, ov);
                 tmem_ld_wait();
-                if (live) {
-                    constexpr int PER = 16 / sizeof(T);
 #pragma unroll
-                    for (int d = 0; d < 32; d += PER) {
-                        alignas(16) T y[PER];
+                for (int d = 0; d < 32; d += PER) {
+                    alignas(16) T y[PER];
 #pragma unroll
-                        for (int e = 0; e < PER; ++e) {  // dimension 4 g + (0, 1, 2, 3) sits at 4 g + (0, 2, 1, 3)
-                            const int at = d + e, w = at & 3;
-                            y[e] = from_f32<T>(__uint_as_float(ov[(at & ~3) + ((w & 1) << 1 | (w >> 1))]) * inv);
-                        }
-                        *reinterpret_cast<uint4*>(dst + 32 * cc + d) = *reinterpret_cast<const uint4*>(y);
+                    for (int e = 0; e < PER; ++e) {  // dimension 4 g + (0, 1, 2, 3) sits at 4 g + (0, 2, 1, 3)
+                        const int at = d + e, w = at & 3;
+                        y[e] = from_f32<T>(__uint_as_float(ov[(at & ~3) + ((w & 1) << 1 | (w >> 1))]) * inv);
                     }
+                    const int ch = (32 * cc + d) / PER;
+                    *reinterpret_cast<uint4*>(own_row + 16 * (ch ^ (row & (CPR - 1)))) = *reinterpret_cast<const uint4*>(y);
                 }
+            }
+            __syncwarp();
+            constexpr int RPP = 32 / CPR;
+            const int64_t own = live ? ((int64_t)(sq.off + tok) * p.H + hq) * HD : -1;
+            const int sub = lane / CPR, ch = lane % CPR;
+#pragma unroll 4
+            for (int b = 0; b < 32 / RPP; ++b) {
+                const int rw = b * RPP + sub, rr = 32 * (warp & 3) + rw;
+                const int64_t at = __shfl_sync(0xffffffffu, own, rw);
+                const uint4 y = *reinterpret_cast<const uint4*>(qs + i * TERMS * TILE + rr * LINE + 16 * (ch ^ (rr & (CPR - 1))));
+                if (at >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at + PER * ch) = y;
             }
         }
     } else if (warp < SM_WARPS + 8) {
@@ -498,8 +536,12 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
                 const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    const uint4 y = make_uint4(bytes_h2<false>(w[2 * hf], false), bytes_h2<false>(w[2 * hf], true),
-                                               bytes_h2<false>(w[2 * hf + 1], false), bytes_h2<false>(w[2 * hf + 1], true));
+                    uint4 y;
+                    if (BF16 && !is_v)
+                        y = make_uint4(bytes_bf2(w[2 * hf]), bytes_bf2(w[2 * hf] >> 8), bytes_bf2(w[2 * hf + 1]), bytes_bf2(w[2 * hf + 1] >> 8));
+                    else
+                        y = make_uint4(bytes_h2<false>(w[2 * hf], false), bytes_h2<false>(w[2 * hf], true),
+                                       bytes_h2<false>(w[2 * hf + 1], false), bytes_h2<false>(w[2 * hf + 1], true));
                     const int cc = (col >> 3) + hf;            // chunk of 8 in atom column i % NA
                     const uint32_t at = is_v ? (r >> 3) * (NA * 1024) + (i % NA) * 1024 + (r & 7) * 128 + ((cc ^ (r & 7)) << 4)
                                              : (i % NA) * ATOM_COL + sw128(r, cc);
