@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
         if constexpr (pr_producer_regs<T>() < pr_launch_regs<T>()) regs_dec<pr_producer_regs<T>()>();
         // Four lanes take 64 bytes of a row, the next four the next row's: in
         // the swizzled tile their 16-byte stores then fall into distinct banks.
-        constexpr int CH = 4 * NA;                     // 16-byte chunks per thread: rows pt / 4 + 32 j, NA chunks of each
+        // A thread has rows pt / 4 + 32 j, NA 16-byte chunks of each.
         const bool is_v = warp >= SM_WARPS + 4;
         const int pt = tid - 32 * SM_WARPS - (is_v ? PR_PRODUCERS : 0);
         const int bmask = (1 << c.lb) - 1, r0 = pt >> 2, col = 16 * (pt & 3);
@@ -507,13 +507,22 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
             return lane < 8 && k < hi && pos < end ? kvb_page(c, sq.slot, pos >> c.lb) : -2;
         };
         const uint32_t slot = smem_u32(raw) + (is_v ? PR_KT * HD : 0) + 16 * pt;  // chunk i at slot + i * 16 * PR_PRODUCERS
-        auto fetch = [&](int k, int page, int i) {     // chunk i of tile k
-            const int r = r0 + 32 * (i / NA), at = k * PR_KT + r;
-            const int pg = __shfl_sync(0xffffffffu, page, r >> 4);
-            const int8_t* from = src + ((((size_t)max(pg, 0) * c.hkv + kvh) << c.lb) + (at & bmask)) * HD + 64 * (i % NA);
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot + i * 16 * PR_PRODUCERS), "l"(from), "r"(at < end && pg >= 0 ? 16 : 0)
-                         : "memory");
+        // rows r0 + 32 j of tile k, into their slots
+        auto fetch = [&](int k, int page, int j) {
+            const int at = k * PR_KT + r0 + 32 * j;
+            const int pg = __shfl_sync(0xffffffffu, page, (r0 >> 4) + 2 * j);
+            const int8_t* from = src + ((((size_t)max(pg, 0) * c.hkv + kvh) << c.lb) + (at & bmask)) * HD;
+            const int n = at < end && pg >= 0 ? 16 : 0;
+#pragma unroll
+            for (int a = 0; a < NA; ++a)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot + (j * NA + a) * 16 * PR_PRODUCERS), "l"(from + 64 * a), "r"(n)
+                             : "memory");
         };
+        // the swizzled place of chunk (j, a): swz[half] + j step_j + a step_a (32 rows keep r & 7)
+        const uint32_t step_j = 4096 * (is_v ? NA : 1), step_a = is_v ? 1024 : ATOM_COL;
+        const uint32_t row_at = (r0 >> 3) * (is_v ? NA * 1024 : 1024) + (r0 & 7) * 128;
+        const uint32_t swz[2] = {row_at + (((col >> 3) ^ (r0 & 7)) << 4), row_at + ((((col >> 3) + 1) ^ (r0 & 7)) << 4)};
+        const uint8_t* mine = raw + (is_v ? PR_KT * HD : 0) + 16 * pt;
         auto scale_of = [&](int page) {
             return page == -1 ? __uint_as_float(0x7FC00000u) : page < 0 ? 0.f : scales[(size_t)page * c.hkv + kvh];
         };
@@ -529,33 +538,36 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
                 if (lane == 0) bar_arrive(&sh.sc_full[sc]);
             }
             uint8_t* dst = (is_v ? vs : ks) + st * TILE;
-#pragma unroll 2
-            for (int i = 0; i < CH; ++i) {
-                const int r = r0 + 32 * (i / NA);
-                const uint4 x = *reinterpret_cast<const uint4*>(raw + (is_v ? PR_KT * HD : 0) + 16 * pt + i * 16 * PR_PRODUCERS);
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            auto convert = [&](auto v_) {
+#pragma unroll 1
+                for (int j = 0; j < 4; ++j) {
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    uint4 y;
-                    if (BF16 && !is_v)
-                        y = make_uint4(bytes_bf2(w[2 * hf]), bytes_bf2(w[2 * hf] >> 8), bytes_bf2(w[2 * hf + 1]), bytes_bf2(w[2 * hf + 1] >> 8));
-                    else
-                        y = make_uint4(bytes_h2<false>(w[2 * hf], false), bytes_h2<false>(w[2 * hf], true),
-                                       bytes_h2<false>(w[2 * hf + 1], false), bytes_h2<false>(w[2 * hf + 1], true));
-                    const int cc = (col >> 3) + hf;            // chunk of 8 in atom column i % NA
-                    const uint32_t at = is_v ? (r >> 3) * (NA * 1024) + (i % NA) * 1024 + (r & 7) * 128 + ((cc ^ (r & 7)) << 4)
-                                             : (i % NA) * ATOM_COL + sw128(r, cc);
-                    *reinterpret_cast<uint4*>(dst + at) = y;
+                    for (int a = 0; a < NA; ++a) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(mine + (j * NA + a) * 16 * PR_PRODUCERS);
+                        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int hf = 0; hf < 2; ++hf) {
+                            uint4 y;
+                            if constexpr (BF16 && !decltype(v_)::value)
+                                y = make_uint4(bytes_bf2(w[2 * hf]), bytes_bf2(w[2 * hf] >> 8), bytes_bf2(w[2 * hf + 1]), bytes_bf2(w[2 * hf + 1] >> 8));
+                            else
+                                y = make_uint4(bytes_h2<false>(w[2 * hf], false), bytes_h2<false>(w[2 * hf], true),
+                                               bytes_h2<false>(w[2 * hf + 1], false), bytes_h2<false>(w[2 * hf + 1], true));
+                            *reinterpret_cast<uint4*>(dst + swz[hf] + j * step_j + a * step_a) = y;
+                        }
+                    }
+                    if (k + 1 < hi) fetch(k + 1, next_page, j);  // into the slots just read
                 }
-                if (k + 1 < hi) fetch(k + 1, next_page, i);  // into the slot just read
-            }
+            };
+            if (BF16 && !is_v) convert(std::false_type{});
+            else convert(std::true_type{});
             fence_async();
             bar_arrive(is_v ? &sh.v_full[st] : &sh.k_full[st]);
             return true;
         };
         int page = lookup(lo), next = lookup(lo + 1);
 #pragma unroll 1
-        for (int i = 0; i < CH; ++i) fetch(lo, page, i);
+        for (int j = 0; j < 4; ++j) fetch(lo, page, j);
         float d = scale_of(page);
         for (int k = lo; k < hi; ++k) {
             const float d_next = scale_of(next);
@@ -580,7 +592,7 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
 #pragma unroll
             for (int e = 0; e < TERMS; ++e) {
                 const uint32_t qd = desc_low(smem_u32(pr_raw) + (i * TERMS + e) * TILE, 1);
-#pragma unroll 1
+#pragma unroll
                 for (int kk = 0; kk < HD / 16; ++kk) {
                     const uint32_t off = ((kk >> 2) * ATOM_COL + 32 * (kk & 3)) >> 4;
                     mma_ss<desc_high(1024), desc_high(1024)>(128 * buf, qd + off, kd + off, IDESC_S, (e > 0 || kk > 0) ? 1u : 0u, leader);
@@ -593,7 +605,7 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
             const uint32_t vd = desc_low(smem_u32(pr_raw) + (NQ * TERMS + 2 + st) * TILE, 64);
 #pragma unroll
             for (int e = 0; e < TERMS; ++e) {
-#pragma unroll 1
+#pragma unroll
                 for (int kk = 0; kk < PR_KT / 16; ++kk)
                     mma_ts<desc_high(NA * 1024)>(T_O + 128 * i, (e == 0 ? 128 * buf : T_LO + 64 * buf) + 8 * kk, vd + ((kk * 2 * (NA * 1024)) >> 4),
                                                  IDESC_O, (e > 0 || kk > 0) ? 1u : acc, leader);
