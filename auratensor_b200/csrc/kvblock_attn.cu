@@ -42,10 +42,12 @@ namespace {
 // F16/BF16 queries are exact in one (each row is scaled by a power of two
 // into f16's range) and their weights are rounded once to 11 bits. The values'
 // scale is part of the weights' exponent: with t_j = s_j + log2 d_v(j) and m
-// their running maximum, P_j = 2^(t_j - m) <= 1 fills f16's range whatever the
-// blocks' scales are; out = sum P_j v8_j / sum P_j / d_v(j).
+// their running maximum, P_j = 2^(t_j - m + 12) fills f16's range whatever the
+// blocks' scales are, and weights down to 2^-26 of the largest keep its full
+// precision; out = sum P_j v8_j / sum P_j / d_v(j).
 constexpr int ST_WARPS = 4;
 constexpr int ST_THREADS = 32 * ST_WARPS;
+constexpr float ST_ROOM = 12.f;
 // Keys of a warp's unit: 8 KB of K and V each at a time. At head_dim 128 a
 // unit of 64 keys needs 252 registers and leaves two warps per scheduler to
 // cover each other's latencies (64 sequences up to 8192 tokens: 163 us); 32
@@ -287,7 +289,7 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 3 : 2) kvb_attn_step_ker
                 l[nt][q] *= a;
                 alpha[nt][q] = a;
                 moved |= a != 1.f;
-                const float sub = mn == -INFINITY ? 0.f : mn - lv;
+                const float sub = mn == -INFINITY ? 0.f : mn - ST_ROOM - lv;
 #pragma unroll
                 for (int j = 0; j < J; ++j)
 #pragma unroll

@@ -14,15 +14,16 @@
 //     with two query tiles one's products run under the other's softmax, with
 //     one (FP32) S has two buffers and the next S runs under this softmax;
 //   a warpgroup per query tile (one thread per row) runs the online softmax:
-//     S from TMEM, twice (its maximum, then the weights: 128 values would not
-//     stay in registers), P back over S's own columns as packed f16.
+//     S from TMEM, P back over S's own columns as packed f16.
 // Arithmetic, per row, in log2 units: t_j = s_j + log2 d_v(j), P_j = 2^(t_j - r)
 // with a reference r that follows the row's largest t; out = sum P_j v8_j /
 // sum P_j / d_v(j). The values' scale is part of the exponent, so P fills
 // f16's range whatever the blocks' scales are, and costs no product; FP32
 // queries keep log2 d_v to its integer part and multiply by the mantissa, as
-// its logarithm is not exact. r is moved (and O, in TMEM, rescaled) only when
-// the maximum outgrows it by 2^8, which f16 holds.
+// its logarithm is not exact. r is set by the maximum of the row's first tile
+// and moves (with O, in TMEM, and what there is of P rescaled) only when 32
+// weights sum to more than f16 may hold: most tiles need no maximum and one
+// pass.
 // FP32 queries take two f16 parts of Q and of P (22 bits) and one query tile.
 // Within a group of 4 head dimensions the f16 order is 0, 2, 1, 3 (how bytes
 // unpack); Q is stored alike and the output is put back in order.
@@ -47,6 +48,11 @@ constexpr int PR_KT = 128;             // keys per tile
 constexpr int PR_ROWS = 128;           // query rows per tile
 constexpr int PR_PRODUCERS = 128;      // for K, and as many for V
 constexpr uint32_t PR_TMEM_COLS = 512;
+// The reference lies 2^8 below a row's maximum when it is set, so that weights
+// down to 2^-22 of the largest keep f16's full precision (FP32 queries: their
+// two parts keep 22 bits down to 2^-11 of it, and 2^-33 of it absolutely); 32
+// weights may sum to 32000 before it moves (times a mantissa: below 65504).
+constexpr float PR_ROOM = 8.f, PR_LIMIT = 32000.f;
 constexpr int kPrSpinLimit = 1 << 20;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -140,6 +146,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
           "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
           "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
           "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -359,9 +372,7 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
             auto tile = [&](auto is_edge) {
                 constexpr bool EDGE = decltype(is_edge)::value;
                 uint32_t x[32];
-                float mx = -INFINITY;
-#pragma unroll 1
-                for (int cc = 0; cc < 4; ++cc) {
+                auto load = [&](int cc) {
                     tmem_ld32(t_s + 32 * cc, x);
                     tmem_ld_wait();
                     if (EDGE) {
@@ -369,6 +380,9 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
                         for (int e = 0; e < 32; ++e)
                             if (32 * cc + e >= hide_from || 32 * cc + e < hide_to) x[e] = 0xFF800000u;
                     }
+                };
+                auto chunk_max = [&](int cc) {  // largest t of the chunk's visible keys
+                    float mx = -INFINITY;
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf) {
                         float m[4];
@@ -380,47 +394,86 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
                         const float t = fmaf(mm, dk[2 * cc + hf] * qf, lv[2 * cc + hf]);
                         mx = fmaxf(mx, EDGE && mm == -INFINITY ? -INFINITY : t);
                     }
+                    return mx;
+                };
+                // rows that have no reference yet take their maximum
+                if (__any_sync(0xffffffffu, r == -INFINITY)) {
+                    float mx = -INFINITY;
+#pragma unroll 1
+                    for (int cc = 0; cc < 4; ++cc) {
+                        load(cc);
+                        mx = fmaxf(mx, chunk_max(cc));
+                    }
+                    if (r == -INFINITY) r = mx - PR_ROOM;
                 }
-                float alpha = 1.f;
-                if (mx > r + 8.f) {
-                    alpha = ex2(r - mx);  // 0 for the first
-                    r = mx;
-                }
-                const float sub = r == -INFINITY ? 0.f : r;
-                float sum = 0.f;
+                float alpha = 1.f, sum = 0.f;
 #pragma unroll 1
                 for (int cc = 0; cc < 4; ++cc) {
                     uint32_t pk[16];
                     [[maybe_unused]] uint32_t pl[16];
-                    tmem_ld32(t_s + 32 * cc, x);
-                    tmem_ld_wait();
+                    load(cc);
+                    float part;
+                    auto weights = [&] {
+                        const float sub = r == -INFINITY ? 0.f : r;
+                        float total = 0.f;
+                        part = 0.f;
 #pragma unroll
-                    for (int hf = 0; hf < 2; ++hf) {
-                        const float f = dk[2 * cc + hf] * qf, off = lv[2 * cc + hf] - sub;
-                        const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
-                        float2 a = make_float2(0.f, 0.f);
+                        for (int hf = 0; hf < 2; ++hf) {
+                            const float f = dk[2 * cc + hf] * qf, off = lv[2 * cc + hf] - sub;
+                            const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
+                            float2 a = make_float2(0.f, 0.f);
 #pragma unroll
-                        for (int e = 0; e < 16; e += 2) {
-                            const int col = 32 * cc + 16 * hf + e;
-                            const float2 t = fma2(make_float2(__uint_as_float(x[16 * hf + e]), __uint_as_float(x[16 * hf + e + 1])), f2, off2);
-                            float2 w = make_float2(ex2(t.x), ex2(t.y));
-                            const bool h0 = EDGE && (col >= hide_from || col < hide_to), h1 = EDGE && (col + 1 >= hide_from || col + 1 < hide_to);
-                            if (EDGE) w = make_float2(h0 ? 0.f : w.x, h1 ? 0.f : w.y);
-                            a = add2(a, w);
-                            if constexpr (TERMS == 2) {
-                                const float m = mv[2 * cc + hf];
-                                w = make_float2(h0 ? 0.f : w.x * m, h1 ? 0.f : w.y * m);
+                            for (int e = 0; e < 16; e += 2) {
+                                const int col = 32 * cc + 16 * hf + e;
+                                const float2 t = fma2(make_float2(__uint_as_float(x[16 * hf + e]), __uint_as_float(x[16 * hf + e + 1])), f2, off2);
+                                float2 w = make_float2(ex2(t.x), ex2(t.y));
+                                const bool h0 = EDGE && (col >= hide_from || col < hide_to), h1 = EDGE && (col + 1 >= hide_from || col + 1 < hide_to);
+                                if (EDGE) w = make_float2(h0 ? 0.f : w.x, h1 ? 0.f : w.y);
+                                a = add2(a, w);
+                                if constexpr (TERMS == 2) {
+                                    const float m = mv[2 * cc + hf];
+                                    w = make_float2(h0 ? 0.f : w.x * m, h1 ? 0.f : w.y * m);
+                                }
+                                const uint32_t h = pack_h2(w.x, w.y);
+                                pk[8 * hf + e / 2] = h;
+                                if constexpr (TERMS == 2) {
+                                    const float2 u = unpack_h2(h);
+                                    pl[8 * hf + e / 2] = pack_h2(w.x - u.x, w.y - u.y);
+                                }
                             }
-                            const uint32_t h = pack_h2(w.x, w.y);
-                            pk[8 * hf + e / 2] = h;
-                            if constexpr (TERMS == 2) {
-                                const float2 u = unpack_h2(h);
-                                pl[8 * hf + e / 2] = pack_h2(w.x - u.x, w.y - u.y);
-                            }
+                            const float as = a.x + a.y;
+                            total += as;
+                            part = EDGE && as == 0.f ? part : fmaf(as, iv[2 * cc + hf], part);
                         }
-                        const float as = a.x + a.y;
-                        sum = EDGE && as == 0.f ? sum : fmaf(as, iv[2 * cc + hf], sum);
+                        return total;
+                    };
+                    // P must stay below f16's largest (times a mantissa): a chunk
+                    // that outgrows the reference moves it, by whole powers of two
+                    const bool over = !(weights() <= PR_LIMIT);  // NaN too, which moves nothing
+                    if (__any_sync(0xffffffffu, over)) {
+                        const float up = over ? fmaxf(ceilf(chunk_max(cc) - PR_ROOM - r), 0.f) : 0.f, a = ex2(-up);
+                        r += up;
+                        alpha *= a;
+                        sum *= a;
+#pragma unroll 1
+                        for (int c2 = 0; c2 < cc; ++c2) {  // what is stored already
+                            auto rescale = [&](uint32_t at) {
+                                uint32_t y[16];
+                                tmem_ld16(at, y);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) {
+                                    const float2 u = unpack_h2(y[e]);
+                                    y[e] = pack_h2(u.x * a, u.y * a);
+                                }
+                                tmem_st16(at, y);
+                            };
+                            rescale(t_s + 16 * c2);
+                            if constexpr (TERMS == 2) rescale(trow + T_LO + 64 * buf + 16 * c2);
+                        }
+                        weights();
                     }
+                    sum += part;
                     // P's columns 16 cc .. are S's columns that have been read
                     tmem_st16(t_s + 16 * cc, pk);
                     if constexpr (TERMS == 2) tmem_st16(trow + T_LO + 64 * buf + 16 * cc, pl);

@@ -437,3 +437,30 @@ def test_reserve_and_release_give_distinct_pages(cuda):
     cache.release(0)
     cache.reserve(2, 96)
     assert cache.freeBlocks() == 0 and not set(cache.table[2].tolist()) & set(cache.table[1, :3].tolist())
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n,step", [(1, 40), (150, 1), (150, 32), (150, 128), (260, 17)])
+def test_scores_that_grow_along_the_keys(n, step, dtype, cuda):
+    """Each `step` keys the scores rise by 12 (in powers of e): the running reference has to follow, inside tiles and
+    across them, and what came before fades without upsetting the sums; in the second half they fall again."""
+    total = 300
+    cache = new_cache(dtype, seqs=1, heads_kv=1, hd=64, block=16, blocks=20, per_seq=20)
+    level = torch.arange(total, device=cuda) // step
+    level = torch.minimum(level, level.max() - level).float() * 12
+    k = heads((total, 1, 64), 91, F32, cuda) * 0.1
+    k[:, 0, 0] = level  # the first dimension alone carries the level
+    k, v = k.to(dtype), heads((total, 1, 64), 92, dtype, cuda)
+    q = heads((n, 4, 64), 93, F32, cuda) * 0.1
+    q[:, :, 0] = 8.0
+    q = q.to(dtype)
+    cache.reserve(0, total)
+    cache.append(0, TokenBatch.of([0], [0], [total]), k, v)
+    y = f64(cache.attention(0, TokenBatch.of([0], [total - n], [n]), q))
+    kd, vd = ref.cache_values(f32(k), 16), ref.cache_values(f32(v), 16)
+    want, mag = ref.attention(f64(q), kd, vd, total - n, 0.125)
+    # a score of size |s| is rounded to FP32 a few times: 2^-22 |s| more on its weight
+    smax = float(np.abs(f64(q)[..., 0]).max() * np.abs(kd[:, 0, 0]).max() * 0.125)
+    tol = (5e-5 + 2.0 ** -21 * smax + (0 if dtype == F32 else 2.0 ** -11)) * mag + ROUND[dtype] * np.abs(want)
+    assert np.all(np.abs(y - want) <= tol), float((np.abs(y - want) / tol).max())
+    cache.check()
