@@ -13,17 +13,19 @@
 //   one thread issues S = Q K^T into TMEM, and O += P V with P read from TMEM;
 //     with two query tiles one's products run under the other's softmax, with
 //     one (FP32) S has two buffers and the next S runs under this softmax;
-//   a warpgroup per query tile (one thread per row) runs the online softmax:
-//     S from TMEM, P back over S's own columns as packed f16.
+//   softmax threads, one per query row with two query tiles, two per row (64
+//     columns of S each, exchanging their maxima) with one: S from TMEM, twice
+//     (its maximum, then the weights: 128 values would not stay in registers),
+//     P back over their own S columns as packed f16. With two tiles two
+//     threads per row were slower (375 us against 344).
 // Arithmetic, per row, in log2 units: t_j = s_j + log2 d_v(j), P_j = 2^(t_j - r)
 // with a reference r that follows the row's largest t; out = sum P_j v8_j /
 // sum P_j / d_v(j). The values' scale is part of the exponent, so P fills
 // f16's range whatever the blocks' scales are, and costs no product; FP32
 // queries keep log2 d_v to its integer part and multiply by the mantissa, as
-// its logarithm is not exact. r is set by the maximum of the row's first tile
-// and moves (with O, in TMEM, and what there is of P rescaled) only when 32
-// weights sum to more than f16 may hold: most tiles need no maximum and one
-// pass.
+// its logarithm is not exact. r is set 2^8 below the row's maximum, and moved
+// (with O, in TMEM, rescaled) only when the maximum outgrows it by 2^14, which
+// f16 holds: weights down to 2^-22 of the largest keep its full precision.
 // FP32 queries take two f16 parts of Q and of P (22 bits) and one query tile.
 // Within a group of 4 head dimensions the f16 order is 0, 2, 1, 3 (how bytes
 // unpack); Q is stored alike and the output is put back in order.
@@ -48,11 +50,7 @@ constexpr int PR_KT = 128;             // keys per tile
 constexpr int PR_ROWS = 128;           // query rows per tile
 constexpr int PR_PRODUCERS = 128;      // for K, and as many for V
 constexpr uint32_t PR_TMEM_COLS = 512;
-// The reference lies 2^8 below a row's maximum when it is set, so that weights
-// down to 2^-22 of the largest keep f16's full precision (FP32 queries: their
-// two parts keep 22 bits down to 2^-11 of it, and 2^-33 of it absolutely); 32
-// weights may sum to 32000 before it moves (times a mantissa: below 65504).
-constexpr float PR_ROOM = 8.f, PR_LIMIT = 32000.f;
+constexpr float PR_ROOM = 8.f, PR_GROW = 14.f;  // the reference lies so far below the maximum; it moves when that outgrows it by so much
 constexpr int kPrSpinLimit = 1 << 20;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -62,9 +60,10 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)_
 // done, which was issued after the softmax of tile k.
 struct PrShared {
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], sc_full[4];
-    uint64_t q_full, s_full[2], p_full[2], pv_done, o_done;
+    uint64_t q_full, s_full[2], p_full[2], pv_done, o_done, pair;  // pair: the two threads of each row
     uint32_t tmem;
     int bad;
+    float top[2][2][PR_ROWS];  // maxima that a row's two threads exchange: [parity of the tile][half][row]
     float dk[4][8], lv[4][8], iv[4][8], mv[4][8];  // per 16 keys: d_k, log2 part and reciprocal of d_v, mantissa
 };
 
@@ -148,13 +147,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
           "=r"(r[31])
         : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-}
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
     asm volatile(
@@ -191,21 +183,25 @@ constexpr int pr_terms() { return sizeof(T) == 4 ? 2 : 1; }
 template <class T>
 constexpr int pr_tiles() { return sizeof(T) == 4 ? 1 : 2; }  // query tiles per CTA
 template <class T>
-constexpr int pr_threads() { return 128 * pr_tiles<T>() + 2 * PR_PRODUCERS + 128; }
+constexpr int pr_halves() { return pr_tiles<T>() == 1 ? 2 : 1; }  // softmax threads per row
+template <class T>
+constexpr int pr_softmax() { return 128 * pr_tiles<T>() * pr_halves<T>(); }
+template <class T>
+constexpr int pr_threads() { return pr_softmax<T>() + 2 * PR_PRODUCERS + 128; }
 // Registers per thread of the softmax, producer and MMA warpgroups. Their sums
 // must stay within what the block is launched with (threads x the compiler's
 // bound for that many): a setmaxnreg.inc beyond it would wait for ever.
 template <class T>
-constexpr int pr_softmax_regs() { return pr_tiles<T>() == 2 ? 112 : 208; }
+constexpr int pr_softmax_regs() { return pr_tiles<T>() == 2 ? 112 : 112; }
 template <class T>
-constexpr int pr_producer_regs() { return pr_tiles<T>() == 2 ? 96 : 112; }
+constexpr int pr_producer_regs() { return pr_tiles<T>() == 2 ? 80 : 80; }
 template <class T>
 constexpr int pr_mma_regs() { return pr_tiles<T>() == 2 ? 56 : 64; }
 template <class T>
 constexpr int pr_launch_regs() { return 65536 / pr_threads<T>() / 8 * 8; }
 template <class T>
 constexpr bool pr_regs_fit() {
-    return 128 * pr_tiles<T>() * pr_softmax_regs<T>() + 2 * PR_PRODUCERS * pr_producer_regs<T>() + 128 * pr_mma_regs<T>() <=
+    return pr_softmax<T>() * pr_softmax_regs<T>() + 2 * PR_PRODUCERS * pr_producer_regs<T>() + 128 * pr_mma_regs<T>() <=
            pr_threads<T>() * pr_launch_regs<T>();
 }
 static_assert(pr_regs_fit<float>() && pr_regs_fit<__half>(), "register shares");
@@ -224,6 +220,8 @@ struct PromptParams {
     float scale;
 };
 
+static_assert(sizeof(PrShared) <= 3072, "what the tiles leave of an SM's 227 KB");
+
 template <class T, int HD>
 __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(const PromptParams p) {
     constexpr int NQ = pr_tiles<T>(), TERMS = pr_terms<T>();
@@ -232,7 +230,7 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
     constexpr uint32_t TILE = 128 * HD * 2;            // bytes of a Q, K or V tile
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     constexpr uint32_t IDESC_S = pr_idesc(PR_ROWS, PR_KT, false, BF16), IDESC_O = pr_idesc(PR_ROWS, HD, true, false);
-    constexpr int SM_WARPS = 4 * NQ;
+    constexpr int HV = pr_halves<T>(), SM_WARPS = pr_softmax<T>() / 32;
     constexpr uint32_t T_O = 256, T_LO = 384;          // TMEM columns: S at 0 and 128, O (per tile), low parts of P (one tile, per buffer)
     extern __shared__ __align__(1024) uint8_t pr_raw[];
     __shared__ PrShared sh;
@@ -275,10 +273,11 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
             bar_init(&sh.sc_full[i], 2);
             bar_init(&sh.sc_full[2 + i], 2);
             bar_init(&sh.s_full[i], 1);
-            bar_init(&sh.p_full[i], 128);
+            bar_init(&sh.p_full[i], 128 * HV);
         }
-        bar_init(&sh.q_full, 128 * NQ);
+        bar_init(&sh.q_full, pr_softmax<T>());
         bar_init(&sh.pv_done, 1);
+        bar_init(&sh.pair, 256);
         bar_init(&sh.o_done, 1);
         sh.bad = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -295,23 +294,24 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
     if (warp < SM_WARPS) {
         // ------------------------------------------------------------ softmax
         regs_inc<pr_softmax_regs<T>()>();
-        const int i = warp >> 2, row = tid & 127;
+        const int i = NQ == 2 ? warp >> 2 : 0, half = HV == 2 ? warp >> 2 : 0, row = tid & 127;
         const uint32_t trow = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t t_o = trow + T_O + 128 * i;
         const int tq = row / p.G, hq = kvh * p.G + row - tq * p.G;  // the row's token of the tile, and its query head
         const int tok = t0 + i * QB + tq;
         const bool live = tq < QB && tok < sq.n;
         const int qpos = live ? start + tok : -1;
+        [[maybe_unused]] float* row_qf = sh.top[1][0];  // FP32 queries: the rows' scaling (free until the second tile)
         float qf = 1.f;  // power of two of the row (FP32 queries), then its score factor, log2 units
         {
             // HD / 8 lanes take a row together (a thread's own row would touch
             // 32 lines per load).
-            constexpr int LPR = HD / 8, RPP = 32 / LPR, PASSES = 32 / RPP, IN_FLIGHT = 8 / TERMS;
+            constexpr int LPR = HD / 8, RPP = 32 / LPR, PASSES = 32 / RPP, IN_FLIGHT = TERMS == 2 || HD == 64 ? 4 : 8;
             const int sub = lane / LPR, d = 8 * (lane % LPR), r_w = 32 * (warp & 3);
             const int64_t own = live ? (int64_t)(sq.off + tok) * p.q_ts + (int64_t)hq * p.q_hs : -1;
             uint8_t* dst = qs + i * TERMS * TILE + (d >> 6) * ATOM_COL;
 #pragma unroll 1
-            for (int b = 0; b < PASSES; b += IN_FLIGHT) {
+            for (int b = half * (PASSES / HV); b < (half + 1) * (PASSES / HV); b += IN_FLIGHT) {
                 Raw8<T> raw8[IN_FLIGHT];
 #pragma unroll
                 for (int j = 0; j < IN_FLIGHT; ++j) {
@@ -336,8 +336,7 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
 #pragma unroll
                         for (int o = LPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                         const float rs = row_scale(top);
-                        const float mine = __shfl_sync(0xffffffffu, rs, (lane % RPP) * LPR);  // of row (b + j) RPP + lane % RPP
-                        if (lane / RPP == b + j) qf = mine;                                    // the row's own thread
+                        if (lane % LPR == 0) row_qf[r_w + (b + j) * RPP + sub] = rs;
                         uint32_t h[4], l[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
@@ -351,14 +350,24 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
                     }
                 }
             }
-            qf = p.scale * 1.44269504088896341f / qf;
             fence_async();
             bar_arrive(&sh.q_full);
         }
-        float r = -INFINITY, l = 0.f;
         bool ok = true;
+        uint32_t pairs = 0;
+        [[maybe_unused]] auto pair_sync = [&] {  // between the two threads of each row; bounded like every wait
+            bar_arrive(&sh.pair);
+            ok = __all_sync(0xffffffffu, bar_wait(&sh.pair, pairs++ & 1, &sh));
+        };
+        if constexpr (TERMS == 2) {
+            pair_sync();
+            qf = row_qf[row];
+        }
+        qf = p.scale * 1.44269504088896341f / qf;
+        float r = -INFINITY, l = 0.f;
         int n = 0;
-        for (int k = max(lo, k_lo[i]); k < k_hi[i]; ++k, ++n) {
+        const int k_first = NQ == 2 && i ? max(lo, k_lo[NQ - 1]) : lo, k_end = NQ == 2 && i ? k_hi[NQ - 1] : k_hi[0];
+        for (int k = k_first; k < k_end && ok; ++k, ++n) {
             const int k0 = k * PR_KT, sc = (k - lo) & 3;
             const int buf = NQ == 2 ? i : n & 1;       // S buffer and its barriers
             const uint32_t t_s = trow + 128 * buf;
@@ -396,86 +405,59 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
                     }
                     return mx;
                 };
-                // rows that have no reference yet take their maximum
-                if (__any_sync(0xffffffffu, r == -INFINITY)) {
-                    float mx = -INFINITY;
+                float mx = -INFINITY;
 #pragma unroll 1
-                    for (int cc = 0; cc < 4; ++cc) {
-                        load(cc);
-                        mx = fmaxf(mx, chunk_max(cc));
-                    }
-                    if (r == -INFINITY) r = mx - PR_ROOM;
+                for (int cc = 4 / HV * half; cc < 4 / HV * (half + 1); ++cc) {
+                    load(cc);
+                    mx = fmaxf(mx, chunk_max(cc));
+                }
+                if constexpr (HV == 2) {
+                    float* share = &sh.top[n & 1][0][row];
+                    share[half * PR_ROWS] = mx;
+                    pair_sync();
+                    if (!ok) return;
+                    mx = fmaxf(mx, share[(half ^ 1) * PR_ROWS]);
                 }
                 float alpha = 1.f, sum = 0.f;
+                if (mx > r + PR_GROW) {
+                    alpha = ex2(r - (mx - PR_ROOM));  // 0 for the first
+                    r = mx - PR_ROOM;
+                }
+                const float sub = r == -INFINITY ? 0.f : r;
 #pragma unroll 1
-                for (int cc = 0; cc < 4; ++cc) {
+                for (int cc = 4 / HV * half; cc < 4 / HV * (half + 1); ++cc) {
                     uint32_t pk[16];
                     [[maybe_unused]] uint32_t pl[16];
                     load(cc);
-                    float part;
-                    auto weights = [&] {
-                        const float sub = r == -INFINITY ? 0.f : r;
-                        float total = 0.f;
-                        part = 0.f;
 #pragma unroll
-                        for (int hf = 0; hf < 2; ++hf) {
-                            const float f = dk[2 * cc + hf] * qf, off = lv[2 * cc + hf] - sub;
-                            const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
-                            float2 a = make_float2(0.f, 0.f);
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const float f = dk[2 * cc + hf] * qf, off = lv[2 * cc + hf] - sub;
+                        const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
+                        float2 a = make_float2(0.f, 0.f);
 #pragma unroll
-                            for (int e = 0; e < 16; e += 2) {
-                                const int col = 32 * cc + 16 * hf + e;
-                                const float2 t = fma2(make_float2(__uint_as_float(x[16 * hf + e]), __uint_as_float(x[16 * hf + e + 1])), f2, off2);
-                                float2 w = make_float2(ex2(t.x), ex2(t.y));
-                                const bool h0 = EDGE && (col >= hide_from || col < hide_to), h1 = EDGE && (col + 1 >= hide_from || col + 1 < hide_to);
-                                if (EDGE) w = make_float2(h0 ? 0.f : w.x, h1 ? 0.f : w.y);
-                                a = add2(a, w);
-                                if constexpr (TERMS == 2) {
-                                    const float m = mv[2 * cc + hf];
-                                    w = make_float2(h0 ? 0.f : w.x * m, h1 ? 0.f : w.y * m);
-                                }
-                                const uint32_t h = pack_h2(w.x, w.y);
-                                pk[8 * hf + e / 2] = h;
-                                if constexpr (TERMS == 2) {
-                                    const float2 u = unpack_h2(h);
-                                    pl[8 * hf + e / 2] = pack_h2(w.x - u.x, w.y - u.y);
-                                }
+                        for (int e = 0; e < 16; e += 2) {
+                            const int col = 32 * cc + 16 * hf + e;
+                            const float2 t = fma2(make_float2(__uint_as_float(x[16 * hf + e]), __uint_as_float(x[16 * hf + e + 1])), f2, off2);
+                            float2 w = make_float2(ex2(t.x), ex2(t.y));
+                            const bool h0 = EDGE && (col >= hide_from || col < hide_to), h1 = EDGE && (col + 1 >= hide_from || col + 1 < hide_to);
+                            if (EDGE) w = make_float2(h0 ? 0.f : w.x, h1 ? 0.f : w.y);
+                            a = add2(a, w);
+                            if constexpr (TERMS == 2) {
+                                const float m = mv[2 * cc + hf];
+                                w = make_float2(h0 ? 0.f : w.x * m, h1 ? 0.f : w.y * m);
                             }
-                            const float as = a.x + a.y;
-                            total += as;
-                            part = EDGE && as == 0.f ? part : fmaf(as, iv[2 * cc + hf], part);
+                            const uint32_t h = pack_h2(w.x, w.y);
+                            pk[8 * hf + e / 2] = h;
+                            if constexpr (TERMS == 2) {
+                                const float2 u = unpack_h2(h);
+                                pl[8 * hf + e / 2] = pack_h2(w.x - u.x, w.y - u.y);
+                            }
                         }
-                        return total;
-                    };
-                    // P must stay below f16's largest (times a mantissa): a chunk
-                    // that outgrows the reference moves it, by whole powers of two
-                    const bool over = !(weights() <= PR_LIMIT);  // NaN too, which moves nothing
-                    if (__any_sync(0xffffffffu, over)) {
-                        const float up = over ? fmaxf(ceilf(chunk_max(cc) - PR_ROOM - r), 0.f) : 0.f, a = ex2(-up);
-                        r += up;
-                        alpha *= a;
-                        sum *= a;
-#pragma unroll 1
-                        for (int c2 = 0; c2 < cc; ++c2) {  // what is stored already
-                            auto rescale = [&](uint32_t at) {
-                                uint32_t y[16];
-                                tmem_ld16(at, y);
-                                tmem_ld_wait();
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) {
-                                    const float2 u = unpack_h2(y[e]);
-                                    y[e] = pack_h2(u.x * a, u.y * a);
-                                }
-                                tmem_st16(at, y);
-                            };
-                            rescale(t_s + 16 * c2);
-                            if constexpr (TERMS == 2) rescale(trow + T_LO + 64 * buf + 16 * c2);
-                        }
-                        weights();
+                        const float as = a.x + a.y;
+                        sum = EDGE && as == 0.f ? sum : fmaf(as, iv[2 * cc + hf], sum);
                     }
-                    sum += part;
-                    // P's columns 16 cc .. are S's columns that have been read
-                    tmem_st16(t_s + 16 * cc, pk);
+                    // over this thread's own S columns, which have been read: 64 columns, or 32 from 0 and from 64
+                    tmem_st16(t_s + (HV == 2 ? 64 * half + 16 * (cc & 1) : 16 * cc), pk);
                     if constexpr (TERMS == 2) tmem_st16(trow + T_LO + 64 * buf + 16 * cc, pl);
                 }
                 l = fmaf(l, alpha, sum);
@@ -488,7 +470,7 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
                     }
                     if (ok) {
 #pragma unroll 1
-                        for (int cc = 0; cc < HD / 32; ++cc) {
+                        for (int cc = half * (HD / 32 / HV); cc < (half + 1) * (HD / 32 / HV); ++cc) {
                             tmem_ld32(t_o + 32 * cc, x);
                             tmem_ld_wait();
 #pragma unroll
@@ -507,15 +489,21 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
         }
         if (ok && n > 0) ok = bar_wait(&sh.o_done, 0, &sh);
         ok = __all_sync(0xffffffffu, ok);
+        if (HV == 2 && ok && n > 0) {
+            float* share = reinterpret_cast<float*>(raw) + row;  // the last tile has left it
+            share[half * PR_ROWS] = l;
+            pair_sync();
+            l = share[0] + share[PR_ROWS];  // in the same order in both
+        }
         if (ok && n > 0) {
             fence_after();
             const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
             // rows go through the query tiles' shared memory (their last product
             // is done) to leave as whole lines; chunks are XOR-swizzled by row
-            constexpr int PER = 16 / sizeof(T), CPR = HD / PER, LINE = HD * (int)sizeof(T);
+            constexpr int PER = 16 / sizeof(T), CPR = HD / PER, LINE = HD * (int)sizeof(T), CPH = CPR / HV;
             uint8_t* own_row = qs + i * TERMS * TILE + row * LINE;
 #pragma unroll 1
-            for (int cc = 0; cc < HD / 32; ++cc) {
+            for (int cc = half * (HD / 32 / HV); cc < (half + 1) * (HD / 32 / HV); ++cc) {
                 uint32_t ov[32];
                 tmem_ld32(t_o + 32 * cc, ov);
                 tmem_ld_wait();
@@ -532,9 +520,9 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
                 }
             }
             __syncwarp();
-            constexpr int RPP = 32 / CPR;
+            constexpr int RPP = 32 / CPH;
             const int64_t own = live ? ((int64_t)(sq.off + tok) * p.H + hq) * HD : -1;
-            const int sub = lane / CPR, ch = lane % CPR;
+            const int sub = lane / CPH, ch = half * CPH + lane % CPH;
 #pragma unroll 4
             for (int b = 0; b < 32 / RPP; ++b) {
                 const int rw = b * RPP + sub, rr = 32 * (warp & 3) + rw;
@@ -660,7 +648,7 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
             for (int e = 0; e < TERMS; ++e) {
 #pragma unroll
                 for (int kk = 0; kk < PR_KT / 16; ++kk)
-                    mma_ts<desc_high(NA * 1024)>(T_O + 128 * i, (e == 0 ? 128 * buf : T_LO + 64 * buf) + 8 * kk, vd + ((kk * 2 * (NA * 1024)) >> 4),
+                    mma_ts<desc_high(NA * 1024)>(T_O + 128 * i, (e == 0 ? 128 * buf + (HV == 2 ? (kk >> 2) * 32 : 0) : T_LO + 64 * buf) + 8 * kk, vd + ((kk * 2 * (NA * 1024)) >> 4),
                                                  IDESC_O, (e > 0 || kk > 0) ? 1u : acc, leader);
             }
         };
