@@ -26,7 +26,7 @@ import torch
 
 from . import _lib
 from ._lib import GGML_BF16, GGML_F16, GGML_F32, IllegalArgumentException, IllegalStateException, KvBlocksC, TokenBatchC, lib
-from .core import context
+from .core import _current_stream, context
 
 DTYPE_CODES = {torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16}
 
@@ -98,33 +98,40 @@ class BlockKvCache:
         self.maxSeqs, self.maxBlocks = table.shape
         self.dtype = dtype
         code = _code(dtype, "the cache's type")
-        scales = (self.layers, self.nBlocks, self.headCountKv)
+        f32 = torch.float32
+        blocks, scales = kBlocks.shape, (self.layers, self.nBlocks, self.headCountKv)
         ring = (self.layers, self.maxSeqs, self.headCountKv, 2 * self.blockTokens)
-        tensors = [(kBlocks, "kBlocks", torch.int8, kBlocks.shape), (vBlocks, "vBlocks", torch.int8, kBlocks.shape),
-                   (kScales, "kScales", torch.float32, scales), (vScales, "vScales", torch.float32, scales)]
-        tails = [(kTail, "kTail", dtype, ring + (self.headDim,)), (vTail, "vTail", dtype, ring + (self.headDim,)),
-                 (kTailMax, "kTailMax", torch.float32, ring), (vTailMax, "vTailMax", torch.float32, ring)]
-        if any(t[0] is not None for t in tails):
-            if any(t[0] is None for t in tails):
-                _bad("kTail, vTail, kTailMax and vTailMax go together")
-            tensors += tails
-        dev = kBlocks.device
-        for t, name, dt, shape in tensors:
+        rows = ring + (self.headDim,)
+        tails = (kTail, vTail, kTailMax, vTailMax)
+        absent = sum(t is None for t in tails)
+        if 0 < absent < 4:
+            _bad("kTail, vTail, kTailMax and vTailMax go together")
+        self.device = kBlocks.device
+        index = self.device.index
+        if not kBlocks.is_cuda or table.get_device() != index or not table.is_contiguous():
+            _bad("the cache must be on one CUDA device, its table contiguous")
+        for t, name, dt, shape in ((kBlocks, "kBlocks", torch.int8, blocks), (vBlocks, "vBlocks", torch.int8, blocks),
+                                   (kScales, "kScales", f32, scales), (vScales, "vScales", f32, scales), (kTail, "kTail", dtype, rows),
+                                   (vTail, "vTail", dtype, rows), (kTailMax, "kTailMax", f32, ring), (vTailMax, "vTailMax", f32, ring)):
+            if t is None and absent == 4:
+                continue
             if t.dtype != dt or t.shape != shape:
                 _bad(f"{name} must be {dt} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-            if t.device != dev or not t.is_contiguous():
+            if t.get_device() != index or not t.is_contiguous():
                 _bad(f"{name} must be contiguous and on the device of kBlocks")
-        if not kBlocks.is_cuda or table.device != dev or not table.is_contiguous():
-            _bad("the cache must be on one CUDA device")
-        self.device = dev
         self.kBlocks, self.vBlocks, self.kScales, self.vScales, self.table = kBlocks, vBlocks, kScales, vScales, table
         self.kTail, self.vTail, self.kTailMax, self.vTailMax, self.status = kTail, vTail, kTailMax, vTailMax, status
         # layer l's buffers start l slices into each tensor
-        per = [(t[0].data_ptr(), t[0].stride(0) * t[0].element_size()) if t[0] is not None else (0, 0)
-               for t in tensors[:4] + tails]
-        shared = (table.data_ptr(), 0 if status is None else status.data_ptr())
+        buffers = (kBlocks, vBlocks, kScales, vScales) + (tails if absent == 0 else ())
+        at = [t.data_ptr() for t in buffers]
+        step = [t.stride(0) * t.element_size() for t in buffers] if self.layers > 1 else None
+        none = (None,) * (8 - len(at))
+        shared = (table.data_ptr(), None if status is None else status.data_ptr())
         self._c = [KvBlocksC(code, self.headCountKv, self.headDim, self.blockTokens, self.nBlocks, self.maxSeqs, self.maxBlocks, 0,
-                             *[(p + l * s) or None for p, s in per], *shared) for l in range(self.layers)]
+                             *(at if l == 0 else [p + l * s for p, s in zip(at, step)]), *none, *shared) for l in range(self.layers)]
+        self._refs = [C.addressof(c) for c in self._c]
+        self._ws: dict = {}  # attention workspaces by stream
+        self._scale = 1.0 / math.sqrt(self.headDim)
         self._free = None
         self._pages = None
 
@@ -203,26 +210,37 @@ class BlockKvCache:
     def _layer(self, layer: int) -> int:
         if not 0 <= layer < self.layers:
             _bad(f"layer {layer} out of range [0, {self.layers})")
-        return C.addressof(self._c[layer])
+        return self._refs[layer]
 
     def _on_device(self, *tensors):
         for t in tensors:
-            if t.device != self.device:
+            if t.get_device() != self.device.index:
                 _bad(f"expected a tensor on {self.device}, got {t.device}")
+
+    def _workspace(self, stream: int, need: int) -> torch.Tensor:
+        """At least `need` bytes that calls on this stream share (they run one
+        after the other). A captured graph gets memory of its own."""
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(need, dtype=torch.uint8, device=self.device)
+        ws = self._ws.get(stream)
+        if ws is None or ws.numel() < need:
+            ws = self._ws[stream] = torch.empty(need, dtype=torch.uint8, device=self.device)
+        return ws
 
     def append(self, layer: int, batch: TokenBatch, k: torch.Tensor, v: torch.Tensor) -> None:
         """Quantizes the batch's K and V ([tokens][kv heads][head dim], the
         cache's dtype; token and head strides are free) into the cache."""
         ref = self._layer(layer)
-        shape = (batch.nTokens, self.headCountKv, self.headDim)
-        for t, name in ((k, "k"), (v, "v")):
+        shape, ks, vs = (batch.nTokens, self.headCountKv, self.headDim), k.stride(), v.stride()
+        for t, s, name in ((k, ks, "k"), (v, vs, "v")):
             if t.dtype != self.dtype or t.shape != shape:
                 _bad(f"{name} must be {self.dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
-            if t.stride(2) != 1:
+            if s[2] != 1:
                 _bad(f"{name}'s last dimension must be contiguous")
         self._on_device(k, v, batch.slots)
-        _lib.check(lib().at_kvb_append(context(self.device.index), ref, batch._ref, k.data_ptr(), k.stride(0), k.stride(1),
-                                       v.data_ptr(), v.stride(0), v.stride(1)))
+        rc = lib().at_kvb_append(context(self.device.index), ref, batch._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1])
+        if rc:
+            _lib.check(rc)
 
     def read(self, layer: int, batch: TokenBatch, dtype: torch.dtype | None = None):
         """K and V of the batch's positions as values, [tokens][kv heads][head dim] each."""
@@ -230,9 +248,11 @@ class BlockKvCache:
         dtype = self.dtype if dtype is None else dtype
         code = _code(dtype, "the output")
         self._on_device(batch.slots)
-        out = torch.empty((2, batch.nTokens, self.headCountKv, self.headDim), dtype=dtype, device=self.device)
-        k, v = out.unbind(0)
-        _lib.check(lib().at_kvb_read(context(self.device.index), ref, batch._ref, code, k.data_ptr(), v.data_ptr()))
+        k = torch.empty((batch.nTokens, self.headCountKv, self.headDim), dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        rc = lib().at_kvb_read(context(self.device.index), ref, batch._ref, code, k.data_ptr(), v.data_ptr())
+        if rc:
+            _lib.check(rc)
         return k, v
 
     def attention(self, layer: int, batch: TokenBatch, q: torch.Tensor, scale: float | None = None, window: int = 0,
@@ -245,21 +265,26 @@ class BlockKvCache:
         if q.dim() != 3 or q.shape[0] != batch.nTokens or q.shape[2] != self.headDim:
             _bad(f"q must be [{batch.nTokens}][heads][{self.headDim}], got {tuple(q.shape)}")
         code = _code(q.dtype, "q")
-        if q.stride(2) != 1:
+        s = q.stride()
+        if s[2] != 1:
             _bad("q's last dimension must be contiguous")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous():
             _bad("out must be contiguous and of q's type and shape")
         self._on_device(q, out, batch.slots)
         heads, window = q.shape[1], int(window)
-        ctx, L = context(self.device.index), lib()
-        need = C.c_size_t()
-        _lib.check(L.at_kvb_attention_workspace(ctx, ref, batch._ref, heads, window, C.byref(need)))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=self.device) if need.value else None
-        _lib.check(L.at_kvb_attention(ctx, ref, batch._ref, code, heads, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(),
-                                      1.0 / math.sqrt(self.headDim) if scale is None else float(scale), window,
-                                      None if ws is None else ws.data_ptr(), need.value))
+        index, L = self.device.index, lib()
+        ctx, need = context(index), C.c_size_t()
+        rc = L.at_kvb_attention_workspace(ctx, ref, batch._ref, heads, window, C.byref(need))
+        if rc:
+            _lib.check(rc)
+        n = need.value
+        ws = self._workspace(_current_stream(index), n).data_ptr() if n else None
+        rc = L.at_kvb_attention(ctx, ref, batch._ref, code, heads, q.data_ptr(), s[0], s[1], out.data_ptr(),
+                                self._scale if scale is None else float(scale), window, ws, n)
+        if rc:
+            _lib.check(rc)
         return out
 
     def check(self) -> None:

@@ -37,19 +37,26 @@ class LogProbs:
         code = _code(logits.dtype, "logits")
         if vocab == 0 or (vocab > 1 and logits.stride(1) != 1):
             raise IllegalArgumentException(_lib.AT_ERR_INVALID_ARG, "logits need a vocabulary, contiguous in memory")
-        dev, f32 = logits.device, torch.float32
+        dev = logits.device
         if tokenIds is not None and (tokenIds.dtype != torch.int32 or tokenIds.shape != (rows,) or tokenIds.device != dev
                                      or not tokenIds.is_contiguous()):
             raise IllegalArgumentException(_lib.AT_ERR_INVALID_ARG, f"tokenIds must be int32 [{rows}] on the logits' device")
         top = int(top)
         if not 0 <= top <= vocab:
             raise IllegalArgumentException(_lib.AT_ERR_INVALID_ARG, f"top must be in [0, {vocab}], got {top}")
-        per_row = torch.empty((3, rows), dtype=f32, device=dev)
-        lse, ent, lp = per_row.unbind(0)
-        ids = torch.empty((rows, top), dtype=torch.int32, device=dev) if top else None
-        alt = torch.empty((rows, top), dtype=f32, device=dev) if top else None
-        _lib.check(lib().at_logprobs(
+        # one allocation: logsumexp, entropy, log probability per row, then the alternatives' ids and log probabilities
+        buf = torch.empty(rows * (3 + 2 * top), dtype=torch.float32, device=dev)
+        lse, ent = buf[:rows], buf[rows:2 * rows]
+        lp = None if tokenIds is None else buf[2 * rows:3 * rows]
+        ids = alt = None
+        at = buf.data_ptr()
+        if top:
+            ids = buf.view(torch.int32).as_strided((rows, top), (top, 1), 3 * rows)
+            alt = buf.as_strided((rows, top), (top, 1), (3 + top) * rows)
+        rc = lib().at_logprobs(
             context(dev.index), logits.data_ptr(), code, rows, vocab, logits.stride(0) if rows > 1 else vocab,
-            None if tokenIds is None else tokenIds.data_ptr(), top, None if tokenIds is None else lp.data_ptr(), lse.data_ptr(),
-            ent.data_ptr(), ids.data_ptr() if top else None, alt.data_ptr() if top else None))
-        return LogProbs(None if tokenIds is None else lp, lse, ent, ids, alt)
+            None if tokenIds is None else tokenIds.data_ptr(), top, None if tokenIds is None else at + 8 * rows, at, at + 4 * rows,
+            at + 12 * rows if top else None, at + 4 * (3 + top) * rows if top else None)
+        if rc:
+            _lib.check(rc)
+        return LogProbs(lp, lse, ent, ids, alt)
