@@ -214,6 +214,18 @@ class LlamaModel:
         n = self.max_batch * self.config.vocabSize
         return _device_view(p.value, n, torch.cuda.current_device()).view(self.max_batch, self.config.vocabSize)
 
+    def logProbs(self, tokenIds=None, top: int = 0) -> "LogProbs":
+        """Log probabilities on the device of the last step's logits rows
+        0..len(tokenIds)-1 (row 0 without tokens): of the given tokens, with
+        the entropy and `top` alternatives (scoring.LogProbs)."""
+        from .scoring import LogProbs
+        rows = 1 if tokenIds is None else len(tokenIds)
+        if not 1 <= rows <= self.max_batch:
+            raise _lib.IllegalArgumentException(_lib.AT_ERR_INVALID_ARG, f"1 to {self.max_batch} rows, got {rows}")
+        logits = self.logitsDevice()[:rows]
+        ids = None if tokenIds is None else torch.as_tensor(tokenIds, dtype=torch.int32).to(logits.device)
+        return LogProbs.of(logits, ids, top)
+
     def generate(self, firstToken: int, startPos: int, nSteps: int, wait: bool = True) -> np.ndarray | None:
         """Greedy decode of slot 0 on the device: nSteps tokens, no host round trip per step."""
         if not wait:
