@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
         const int tq = row / p.G, hq = kvh * p.G + row - tq * p.G;  // the row's token of the tile, and its query head
         const int tok = t0 + i * QB + tq;
         const bool live = tq < QB && tok < sq.n;
-        const int qpos = live ? start + tok : -1;
+        const int qpos = start + min(tok, min(sq.n, t0 + (i + 1) * QB) - 1);  // padding rows: the last row's, so that they need no edge of their own
         [[maybe_unused]] float* row_qf = sh.top[1][0];  // FP32 queries: the rows' scaling (free until the second tile)
         float qf = 1.f;  // power of two of the row (FP32 queries), then its score factor, log2 units
         {
@@ -381,17 +381,20 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
             auto tile = [&](auto is_edge) {
                 constexpr bool EDGE = decltype(is_edge)::value;
                 uint32_t x[32];
+                [[maybe_unused]] uint32_t sees = ~0u;  // the chunk's visible columns, a bit each
+                auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };
                 auto load = [&](int cc) {
                     tmem_ld32(t_s + 32 * cc, x);
+                    if (EDGE) sees = below(hide_from - 32 * cc) & ~below(hide_to - 32 * cc);
                     tmem_ld_wait();
-                    if (EDGE) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (32 * cc + e >= hide_from || 32 * cc + e < hide_to) x[e] = 0xFF800000u;
-                    }
                 };
                 auto chunk_max = [&](int cc) {  // largest t of the chunk's visible keys
                     float mx = -INFINITY;
+                    if (EDGE) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!(sees & (1u << e))) x[e] = 0xFF800000u;
+                    }
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf) {
                         float m[4];
@@ -436,11 +439,9 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
                         float2 a = make_float2(0.f, 0.f);
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {
-                            const int col = 32 * cc + 16 * hf + e;
+                            const bool h0 = EDGE && !(sees & (1u << (16 * hf + e))), h1 = EDGE && !(sees & (2u << (16 * hf + e)));
                             const float2 t = fma2(make_float2(__uint_as_float(x[16 * hf + e]), __uint_as_float(x[16 * hf + e + 1])), f2, off2);
-                            float2 w = make_float2(ex2(t.x), ex2(t.y));
-                            const bool h0 = EDGE && (col >= hide_from || col < hide_to), h1 = EDGE && (col + 1 >= hide_from || col + 1 < hide_to);
-                            if (EDGE) w = make_float2(h0 ? 0.f : w.x, h1 ? 0.f : w.y);
+                            float2 w = make_float2(ex2(h0 ? -INFINITY : t.x), ex2(h1 ? -INFINITY : t.y));
                             a = add2(a, w);
                             if constexpr (TERMS == 2) {
                                 const float m = mv[2 * cc + hf];
