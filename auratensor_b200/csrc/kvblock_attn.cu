@@ -49,13 +49,22 @@ namespace cg = cooperative_groups;
 // their running maximum, P_j = 2^(t_j - m + 12) fills f16's range whatever the
 // blocks' scales are, and weights down to 2^-26 of the largest keep its full
 // precision; out = sum P_j v8_j / sum P_j / d_v(j).
+//
+// 64 sequences of 4096 to 8191 tokens, 64 BF16 heads over 8 of 128: 149 us, 5.3
+// TB/s of K and V, four fifths of a copy's rate: half of the issue slots and
+// 58 % of the integer pipe go to turning bytes into f16, with 12 warps per SM
+// to cover the loads. (K Q^T on the int8 form of mma.sync, with no work per key
+// byte: 142 us with queries as two int8 parts, which lose what is small beside
+// a row's largest value; 148 us with three, which do not.) One sequence of
+// 131072 tokens over 8 heads of 64: 38 us, 3.5 TB/s; of 513 tokens: 7.3 us, the
+// time of its launch and of three loads one after another.
 constexpr int ST_WARPS = 4;
 constexpr int ST_THREADS = 32 * ST_WARPS;
 constexpr float ST_ROOM = 12.f;
 // Keys of a warp's unit: 8 KB of K and V each at a time. At head_dim 128 a
 // unit of 64 keys needs 252 registers and leaves two warps per scheduler to
-// cover each other's latencies (64 sequences up to 8192 tokens: 163 us); 32
-// keys fit 168 registers and three.
+// cover each other's latencies (64 sequences up to 8191 tokens: 163 us); 32
+// keys fit 168 registers and three (149 us).
 constexpr int st_unit(int hd) { return hd == 128 ? 32 : 64; }
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -526,10 +535,10 @@ struct StepPlan {
 
 // Splits along the keys. Three CTAs are resident per SM (two for 16 rows).
 // Fewer items than that: as many splits as fill the GPU once (more only
-// lengthen the join: one sequence of 131072 tokens, 8 KV heads of 64: 40 us
+// lengthen the join: one sequence of 131072 tokens, 8 KV heads of 64: 38 us
 // at 1 wave, 51 at 3). More items: several waves, because sequences differ in
-// length (64 sequences of 4096 to 8192 tokens: 192 us unsplit at 1.2 waves,
-// 153 at 3.5). A split keeps at least one unit per warp.
+// length (64 sequences of 4096 to 8191 tokens: 187 us at 2 waves, 148 to 156
+// from 2.5 to 9, 157 at 16). A split keeps at least one unit per warp.
 StepPlan step_plan(const at_ctx* ctx, const KvbDev& c, const KvbBatch& b, int64_t max_end, int n_heads, int window, int max_rows) {
     const int G = n_heads / c.hkv;
     const int most = (int)std::min<int64_t>((int64_t)b.max_tokens * G, max_rows);
@@ -547,7 +556,7 @@ StepPlan step_plan(const at_ctx* ctx, const KvbDev& c, const KvbBatch& b, int64_
     // 2, 4 or 8 CTAs) and need neither workspace nor a second launch (one
     // sequence of 513 tokens: 10.4 -> 7.3 us). In several waves a cluster's
     // CTAs hold their places until the last is done (64 sequences: 163 us
-    // against 155 with the join as a kernel).
+    // against 149 with the join as a kernel).
     const int pow2 = s.splits <= 2 ? s.splits : s.splits <= 4 ? 4 : 8;
     s.cluster = s.splits > 1 && s.splits <= 8 && items * pow2 <= slots;
     if (s.cluster) s.splits = pow2;
@@ -589,7 +598,7 @@ constexpr int STEP_MAX_ROWS = 64;
 // The step kernel serves every sequence of at most STEP_MAX_ROWS query rows
 // per KV head; it is left out when the host's sizes say that there is none.
 bool uses_step(const KvbBatch& b, int G) {
-    return b.max_tokens * G <= STEP_MAX_ROWS || (int64_t)b.n_seqs * b.max_tokens > b.n_tokens;
+    return (int64_t)b.max_tokens * G <= STEP_MAX_ROWS || (int64_t)b.n_seqs * b.max_tokens > b.n_tokens;
 }
 
 }  // namespace
@@ -645,7 +654,7 @@ int at_kvb_attention(at_ctx* ctx, const at_kvb* cache, const at_token_batch* bat
                 else launch_step<T, 64>(p, s, ctx->stream);
             });
         }
-        if (b.max_tokens * (n_heads / c.hkv) > STEP_MAX_ROWS)
+        if ((int64_t)b.max_tokens * (n_heads / c.hkv) > STEP_MAX_ROWS)
             launch_kvb_attn_prompt(c, b, dtype, n_heads, q, q_token_stride, q_head_stride, out, scale, window, STEP_MAX_ROWS, ctx->stream);
     });
 }

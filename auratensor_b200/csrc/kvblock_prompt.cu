@@ -8,8 +8,9 @@
 //   two warpgroups of producers, one for K and one for V, copy a tile's int8
 //     rows from their pages into shared memory (cp.async, each thread its own
 //     chunks: the next tile's are in flight while this one's are converted),
-//     turn them into f16 (exact, |q| <= 127) and store them into a two-stage
-//     ring: K K-major, V MN-major, 128-byte swizzle;
+//     turn them into f16, or K into bf16 for BF16 queries (both exact,
+//     |q| <= 127), and store them into a two-stage ring: K K-major, V MN-major,
+//     128-byte swizzle;
 //   one thread issues S = Q K^T into TMEM, and O += P V with P read from TMEM;
 //     with two query tiles one's products run under the other's softmax, with
 //     one (FP32) S has two buffers and the next S runs under this softmax;
@@ -17,7 +18,7 @@
 //     columns of S each, exchanging their maxima) with one: S from TMEM, twice
 //     (its maximum, then the weights: 128 values would not stay in registers),
 //     P back over their own S columns as packed f16. With two tiles two
-//     threads per row were slower (375 us against 344).
+//     threads per row were slower (375 us where one takes 344).
 // Arithmetic, per row, in log2 units: t_j = s_j + log2 d_v(j), P_j = 2^(t_j - r)
 // with a reference r that follows the row's largest t; out = sum P_j v8_j /
 // sum P_j / d_v(j). The values' scale is part of the exponent, so P fills
@@ -29,10 +30,20 @@
 // FP32 queries take two f16 parts of Q and of P (22 bits) and one query tile.
 // Within a group of 4 head dimensions the f16 order is 0, 2, 1, 3 (how bytes
 // unpack); Q is stored alike and the output is put back in order.
-// The loops are kept short on purpose (unrolled over 32 columns or one chunk,
-// not over a tile): the roles together run far apart in the code, and with
-// tiles unrolled the instruction cache did not hold them (2 prompts up to 4096
-// tokens: 505 us, the MMA warp at 130 cycles per instruction).
+//
+// Two prompts up to 4096 tokens, 32 BF16 heads over 8 of 128: 320 us, 727
+// TFLOP/s of causal products, 45 % of a plain matrix product's rate; 512
+// tokens in FP32 (three products for one): 18 us. What bounds it: a tile of
+// 128 x 128 weights costs 1024 cycles of ex2 and 1024 of tensor work, and a
+// query tile's softmax, P V and next S follow one another (4500 cycles for two
+// tiles); 15 % of a block's time is its first loads and its last stores.
+// S in two buffers of 64 keys breaks that chain but pays for each product as
+// for one of 128 (415 us); releasing P in halves holds up the other tile's
+// products (332 us).
+// The loops are kept short on purpose (unrolled over 32 columns or one chunk):
+// five roles run apart in the code and share the instruction caches. The
+// conversion unrolled by four: 337 us; the weights of 128 columns straight on,
+// though they save a TMEM load: 347 us.
 // Every wait is bounded: one that runs out sets the status bit, and all roles
 // leave.
 #include <cstdint>
@@ -100,8 +111,9 @@ __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.
 // The MMA warp runs as a whole, with operands that the compiler knows to be
 // the same in every lane (tile addresses are constants of the block, TMEM
 // addresses literals): they then live in uniform registers, where the
-// instruction wants them. From general registers an MMA took 110 to 150 cycles
-// to issue, twice its 64 on the tensor cores. Only the leader's executes.
+// instruction wants them. Issued by one elected thread with operands of its
+// own, an MMA took 110 to 150 cycles, twice its 64 on the tensor cores. Only
+// the leader's executes.
 __device__ __forceinline__ void mma_commit(uint64_t* bar, uint32_t leader) {
     asm volatile(
         "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
@@ -192,11 +204,11 @@ constexpr int pr_threads() { return pr_softmax<T>() + 2 * PR_PRODUCERS + 128; }
 // must stay within what the block is launched with (threads x the compiler's
 // bound for that many): a setmaxnreg.inc beyond it would wait for ever.
 template <class T>
-constexpr int pr_softmax_regs() { return pr_tiles<T>() == 2 ? 112 : 112; }
+constexpr int pr_softmax_regs() { return 112; }
 template <class T>
-constexpr int pr_producer_regs() { return pr_tiles<T>() == 2 ? 80 : 80; }
+constexpr int pr_producer_regs() { return 80; }
 template <class T>
-constexpr int pr_mma_regs() { return pr_tiles<T>() == 2 ? 56 : 64; }
+constexpr int pr_mma_regs() { return 56; }
 template <class T>
 constexpr int pr_launch_regs() { return 65536 / pr_threads<T>() / 8 * 8; }
 template <class T>
@@ -306,7 +318,7 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
         {
             // HD / 8 lanes take a row together (a thread's own row would touch
             // 32 lines per load).
-            constexpr int LPR = HD / 8, RPP = 32 / LPR, PASSES = 32 / RPP, IN_FLIGHT = TERMS == 2 || HD == 64 ? 4 : 8;
+            constexpr int LPR = HD / 8, RPP = 32 / LPR, PASSES = 32 / RPP, IN_FLIGHT = TERMS == 2 ? 4 : PASSES;
             const int sub = lane / LPR, d = 8 * (lane % LPR), r_w = 32 * (warp & 3);
             const int64_t own = live ? (int64_t)(sq.off + tok) * p.q_ts + (int64_t)hq * p.q_hs : -1;
             uint8_t* dst = qs + i * TERMS * TILE + (d >> 6) * ATOM_COL;

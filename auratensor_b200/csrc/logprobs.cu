@@ -19,8 +19,14 @@
 // its own lanes' maxima, so that a row whose large logits come late does not
 // flood the list. Ties: tau is set just below its value, so that the logits
 // equal to it are listed, unless there are many (constant or masked rows);
-// then they are left out and the first ids equal to tau fill up at the end. A row is one CTA, or a cluster of up to 8 whose parts meet in distributed
+// then they are left out and the first ids equal to tau fill up at the end. A
+// row is one CTA, or a cluster of up to 8 whose parts meet in distributed
 // shared memory when there are too few rows to fill the GPU.
+// 2048 rows of 128256 logits, k = 20: 138 us in BF16 (3.8 TB/s; the sums and the
+// comparison with tau cost more than the loads), 183 us in FP32 (5.7 TB/s). 8
+// rows of FP32, k = 5: 8.4 us, its launch, the list's ranking and the cluster's
+// join. 256 threads are as fast for many rows and slower for few (10.5 us); the
+// next step's loads ahead of time need 64 registers and lose a CTA (167 us).
 #include <cooperative_groups.h>
 
 #include <cstdint>

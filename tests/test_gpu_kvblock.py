@@ -464,3 +464,40 @@ def test_scores_that_grow_along_the_keys(n, step, dtype, cuda):
     tol = (5e-5 + 2.0 ** -21 * smax + (0 if dtype == F32 else 2.0 ** -11)) * mag + ROUND[dtype] * np.abs(want)
     assert np.all(np.abs(y - want) <= tol), float((np.abs(y - want) / tol).max())
     cache.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n,hd", [(1, 128), (3, 64), (150, 128), (70, 64)])
+def test_queries_with_one_large_component(n, hd, dtype, cuda):
+    """A component of 4096 that meets zero keys adds nothing, and what stands beside it (0.25 and more of 1) keeps its
+    digits: the row is scaled as a whole, and its other components still lie 2^13 above where f16 ends."""
+    total = 200
+    cache = new_cache(dtype, seqs=1, heads_kv=2, hd=hd, block=32, blocks=8, per_seq=8)
+    k, v = heads((total, 2, hd), 95, dtype, cuda), heads((total, 2, hd), 96, dtype, cuda)
+    k[:, :, 5] = 0
+    q = heads((n, 8, hd), 97, F32, cuda)
+    q = torch.where(q >= 0, q + 0.25, q - 0.25)
+    q[:, :, 5] = torch.where(q[:, :, 5] > 0, 4096.0, -4096.0)
+    q = q.to(dtype)
+    cache.reserve(0, total)
+    cache.append(0, TokenBatch.of([0], [0], [total]), k, v)
+    y = f64(cache.attention(0, TokenBatch.of([0], [total - n], [n]), q))
+    want, mag = ref.attention(f64(q), ref.cache_values(f32(k), 32), ref.cache_values(f32(v), 32), total - n, hd ** -0.5)
+    tol = (5e-5 + (0 if dtype == F32 else 2.0 ** -11)) * mag + ROUND[dtype] * np.abs(want)
+    assert np.all(np.abs(y - want) <= tol), float((np.abs(y - want) / tol).max())
+    cache.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("window", [0, 33])
+@pytest.mark.parametrize("group,n", [(3, 100), (48, 5), (100, 2), (128, 3)])
+def test_query_tiles_with_padding_rows(group, n, window, dtype, cuda):
+    """Groups that leave rows of a tile without a token, and last tiles that are not full."""
+    run_attention(cuda, dtype, 64, 32, 1, group, [(130, n), (0, n + 1)], window=window, seed=group)
+
+
+def test_more_query_heads_than_a_tile_has_rows_are_refused(cuda):
+    cache = new_cache(F16, seqs=1, heads_kv=1, hd=64, block=16, blocks=4, per_seq=4)
+    cache.reserve(0, 1)
+    with pytest.raises(_lib.UnsupportedOperationException, match="128 query heads"):
+        cache.attention(0, TokenBatch.of([0], [0], [1]), heads((1, 129, 64), 1, F16, cuda))
