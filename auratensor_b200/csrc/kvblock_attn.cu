@@ -56,7 +56,7 @@ namespace cg = cooperative_groups;
 // to cover the loads. (K Q^T on the int8 form of mma.sync, with no work per key
 // byte: 142 us with queries as two int8 parts, which lose what is small beside
 // a row's largest value; 148 us with three, which do not.) One sequence of
-// 131072 tokens over 8 heads of 64: 38 us, 3.5 TB/s; of 513 tokens: 7.3 us, the
+// 131072 tokens over 8 heads of 64: 39 us, 3.4 TB/s; of 513 tokens: 7.6 us, the
 // time of its launch and of three loads one after another.
 constexpr int ST_WARPS = 4;
 constexpr int ST_THREADS = 32 * ST_WARPS;
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 3 : 2) kvb_attn_step_ker
         const bool whole = u * UNIT + UNIT - 1 <= first_pos && (p.window <= 0 || u * UNIT > last_pos - p.window);
         float lv, iv, mv;
         value_scale<!BIASED>(dv_u, &lv, &iv, &mv);
-        bool moved = false;
+        [[maybe_unused]] bool moved = false;
         float alpha[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -335,47 +335,84 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 3 : 2) kvb_attn_step_ker
                     if (!whole) hide();
                 }
             }
-        if (__any_sync(0xffffffffu, moved)) {
+        // O^T = O^T alpha + V^T P^T. The tensor cores truncate what they
+        // accumulate: each product in a chain loses some 10^-8 of the sum. FP32
+        // queries therefore start each unit's product from zero and add it in
+        // FP32 (150 sequences of 8000 tokens: 0.7e-6 off instead of 3.5e-6). The
+        // 2000 products of a 16-bit warp over 131072 keys lose 2e-5, a tenth of
+        // what rounding to F16 does, and the additions would cost an eighth of
+        // the time (169 us instead of 149).
+        if constexpr (TERMS == 2) {
+            uint32_t pf[J][NT][TERMS][2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int j = 0; j < J; ++j)
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    o[nt][i][0] *= alpha[nt][0];
-                    o[nt][i][1] *= alpha[nt][1];
-                    o[nt][i][2] *= alpha[nt][0];
-                    o[nt][i][3] *= alpha[nt][1];
-                }
-        }
-        // O^T += V^T P^T
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            uint32_t pf[NT][TERMS][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float a = sc[j][nt][2 * e], b = sc[j][nt][2 * e + 1];
-                    const uint32_t h = pack_h2(a, b);
-                    pf[nt][0][e] = transpose8(h);
-                    if constexpr (TERMS == 2) {
+                    for (int e = 0; e < 2; ++e) {
+                        const float a = sc[j][nt][2 * e], b = sc[j][nt][2 * e + 1];
+                        const uint32_t h = pack_h2(a, b);
                         const float2 f = unpack_h2(h);
-                        pf[nt][1][e] = transpose8(pack_h2(a - f.x, b - f.y));
+                        pf[j][nt][0][e] = transpose8(h);
+                        pf[j][nt][1][e] = transpose8(pack_h2(a - f.x, b - f.y));
                     }
-                }
 #pragma unroll
-            for (int w = 0; w < VB / 4; ++w) {
-                uint32_t x[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = vr[j][e].w[w];
+            for (int w = 0; w < VB / 4; ++w)
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {  // dims 4 w + 2 hf, + 1 of the lane's VB
-                    const uint32_t k01 = __byte_perm(x[0], x[1], hf ? 0x7632 : 0x5410), k23 = __byte_perm(x[2], x[3], hf ? 0x7632 : 0x5410);
-                    const uint32_t a0 = bytes_h2<false>(k01, false), a1 = bytes_h2<false>(k01, true);
-                    const uint32_t a2 = bytes_h2<false>(k23, false), a3 = bytes_h2<false>(k23, true);
+                    float part[NT][4] = {};
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                    for (int j = 0; j < J; ++j) {
+                        const uint32_t k01 = __byte_perm(vr[j][0].w[w], vr[j][1].w[w], hf ? 0x7632 : 0x5410);
+                        const uint32_t k23 = __byte_perm(vr[j][2].w[w], vr[j][3].w[w], hf ? 0x7632 : 0x5410);
+                        const uint32_t a0 = bytes_h2<false>(k01, false), a1 = bytes_h2<false>(k01, true);
+                        const uint32_t a2 = bytes_h2<false>(k23, false), a3 = bytes_h2<false>(k23, true);
 #pragma unroll
-                        for (int e = 0; e < TERMS; ++e) mma16816(o[nt][2 * w + hf], a0, a1, a2, a3, pf[nt][e][0], pf[nt][e][1]);
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = TERMS - 1; e >= 0; --e) mma16816(part[nt], a0, a1, a2, a3, pf[j][nt][e][0], pf[j][nt][e][1]);
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float* y = o[nt][2 * w + hf];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y[e] = fmaf(y[e], alpha[nt][e & 1], part[nt][e]);
+                    }
+                }
+        } else {
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        o[nt][i][0] *= alpha[nt][0];
+                        o[nt][i][1] *= alpha[nt][1];
+                        o[nt][i][2] *= alpha[nt][0];
+                        o[nt][i][3] *= alpha[nt][1];
+                    }
+            }
+            // O^T += V^T P^T
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                uint32_t pf[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        pf[nt][e] = transpose8(pack_h2(sc[j][nt][2 * e], sc[j][nt][2 * e + 1]));
+#pragma unroll
+                for (int w = 0; w < VB / 4; ++w) {
+                    uint32_t x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = vr[j][e].w[w];
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {  // dims 4 w + 2 hf, + 1 of the lane's VB
+                        const uint32_t k01 = __byte_perm(x[0], x[1], hf ? 0x7632 : 0x5410), k23 = __byte_perm(x[2], x[3], hf ? 0x7632 : 0x5410);
+                        const uint32_t a0 = bytes_h2<false>(k01, false), a1 = bytes_h2<false>(k01, true);
+                        const uint32_t a2 = bytes_h2<false>(k23, false), a3 = bytes_h2<false>(k23, true);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][2 * w + hf], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
+                    }
                 }
             }
         }
@@ -535,7 +572,7 @@ struct StepPlan {
 
 // Splits along the keys. Three CTAs are resident per SM (two for 16 rows).
 // Fewer items than that: as many splits as fill the GPU once (more only
-// lengthen the join: one sequence of 131072 tokens, 8 KV heads of 64: 38 us
+// lengthen the join: one sequence of 131072 tokens, 8 KV heads of 64: 39 us
 // at 1 wave, 51 at 3). More items: several waves, because sequences differ in
 // length (64 sequences of 4096 to 8191 tokens: 187 us at 2 waves, 148 to 156
 // from 2.5 to 9, 157 at 16). A split keeps at least one unit per warp.

@@ -28,12 +28,17 @@
 // (with O, in TMEM, rescaled) only when the maximum outgrows it by 2^14, which
 // f16 holds: weights down to 2^-22 of the largest keep its full precision.
 // FP32 queries take two f16 parts of Q and of P (22 bits) and one query tile.
+// The tensor cores truncate what they accumulate, so each product in a chain
+// loses some 10^-8 of the sum: for FP32 queries O leaves TMEM after every key
+// tile and is added in FP32 registers (128 tokens behind 30000: 7e-5 off
+// before). 16-bit queries keep it in TMEM, where 131072 keys lose 3e-4, as
+// much as half the last place of F16.
 // Within a group of 4 head dimensions the f16 order is 0, 2, 1, 3 (how bytes
 // unpack); Q is stored alike and the output is put back in order.
 //
-// Two prompts up to 4096 tokens, 32 BF16 heads over 8 of 128: 320 us, 727
+// Two prompts up to 4096 tokens, 32 BF16 heads over 8 of 128: 321 us, 725
 // TFLOP/s of causal products, 45 % of a plain matrix product's rate; 512
-// tokens in FP32 (three products for one): 18 us. What bounds it: a tile of
+// tokens in FP32 (two products for one): 19 us. What bounds it: a tile of
 // 128 x 128 weights costs 1024 cycles of ex2 and 1024 of tensor work, and a
 // query tile's softmax, P V and next S follow one another (4500 cycles for two
 // tiles); 15 % of a block's time is its first loads and its last stores.
@@ -204,11 +209,11 @@ constexpr int pr_threads() { return pr_softmax<T>() + 2 * PR_PRODUCERS + 128; }
 // must stay within what the block is launched with (threads x the compiler's
 // bound for that many): a setmaxnreg.inc beyond it would wait for ever.
 template <class T>
-constexpr int pr_softmax_regs() { return 112; }
+constexpr int pr_softmax_regs() { return pr_tiles<T>() == 2 ? 112 : 144; }
 template <class T>
-constexpr int pr_producer_regs() { return 80; }
+constexpr int pr_producer_regs() { return pr_tiles<T>() == 2 ? 80 : 72; }
 template <class T>
-constexpr int pr_mma_regs() { return 56; }
+constexpr int pr_mma_regs() { return pr_tiles<T>() == 2 ? 56 : 40; }
 template <class T>
 constexpr int pr_launch_regs() { return 65536 / pr_threads<T>() / 8 * 8; }
 template <class T>
@@ -376,8 +381,20 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
             qf = row_qf[row];
         }
         qf = p.scale * 1.44269504088896341f / qf;
-        float r = -INFINITY, l = 0.f;
+        float r = -INFINITY, l = 0.f, alpha = 1.f;
+        [[maybe_unused]] float acc[NQ == 1 ? HD / HV : 1] = {};  // one query tile: this thread's part of O
         int n = 0;
+        // acc = (acc + the last tile's product) f
+        [[maybe_unused]] auto collect = [&](float f) {
+#pragma unroll
+            for (int cc = 0; cc < (int)(sizeof(acc) / sizeof(float)) / 32; ++cc) {
+                uint32_t y[32];
+                tmem_ld32(t_o + half * (HD / HV) + 32 * cc, y);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) acc[32 * cc + e] = (acc[32 * cc + e] + __uint_as_float(y[e])) * f;
+            }
+        };
         const int k_first = NQ == 2 && i ? max(lo, k_lo[NQ - 1]) : lo, k_end = NQ == 2 && i ? k_hi[NQ - 1] : k_hi[0];
         for (int k = k_first; k < k_end && ok; ++k, ++n) {
             const int k0 = k * PR_KT, sc = (k - lo) & 3;
@@ -433,7 +450,8 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
                     if (!ok) return;
                     mx = fmaxf(mx, share[(half ^ 1) * PR_ROWS]);
                 }
-                float alpha = 1.f, sum = 0.f;
+                float sum = 0.f;
+                alpha = 1.f;
                 if (mx > r + PR_GROW) {
                     alpha = ex2(r - (mx - PR_ROOM));  // 0 for the first
                     r = mx - PR_ROOM;
@@ -474,28 +492,28 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
                     if constexpr (TERMS == 2) tmem_st16(trow + T_LO + 64 * buf + 16 * cc, pl);
                 }
                 l = fmaf(l, alpha, sum);
-                if (n > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-                    // O of the earlier tiles must be complete: with two query
-                    // tiles its product was issued before this S
-                    if (NQ == 1) {
-                        ok = __all_sync(0xffffffffu, bar_wait(&sh.pv_done, (n - 1) & 1, &sh));
-                        fence_after();
-                    }
-                    if (ok) {
+                // with two query tiles O stays in TMEM; its last product was issued before this S
+                if (NQ == 2 && n > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll 1
-                        for (int cc = half * (HD / 32 / HV); cc < (half + 1) * (HD / 32 / HV); ++cc) {
-                            tmem_ld32(t_o + 32 * cc, x);
-                            tmem_ld_wait();
+                    for (int cc = 0; cc < HD / 32; ++cc) {
+                        tmem_ld32(t_o + 32 * cc, x);
+                        tmem_ld_wait();
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * alpha);
-                            tmem_st32(t_o + 32 * cc, x);
-                        }
+                        for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * alpha);
+                        tmem_st32(t_o + 32 * cc, x);
                     }
                 }
             };
             if (edge) tile(std::true_type{});
             else tile(std::false_type{});
             if (!ok) break;
+            if constexpr (NQ == 1) {
+                if (n > 0) {
+                    if (!(ok = __all_sync(0xffffffffu, bar_wait(&sh.pv_done, (n - 1) & 1, &sh)))) break;
+                    fence_after();
+                    collect(alpha);
+                }
+            }
             tmem_st_wait();
             fence_before();
             bar_arrive(&sh.p_full[buf]);
@@ -515,11 +533,7 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
             // is done) to leave as whole lines; chunks are XOR-swizzled by row
             constexpr int PER = 16 / sizeof(T), CPR = HD / PER, LINE = HD * (int)sizeof(T), CPH = CPR / HV;
             uint8_t* own_row = qs + i * TERMS * TILE + row * LINE;
-#pragma unroll 1
-            for (int cc = half * (HD / 32 / HV); cc < (half + 1) * (HD / 32 / HV); ++cc) {
-                uint32_t ov[32];
-                tmem_ld32(t_o + 32 * cc, ov);
-                tmem_ld_wait();
+            auto put = [&](int cc, const uint32_t* ov) {
 #pragma unroll
                 for (int d = 0; d < 32; d += PER) {
                     alignas(16) T y[PER];
@@ -530,6 +544,19 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
                     }
                     const int ch = (32 * cc + d) / PER;
                     *reinterpret_cast<uint4*>(own_row + 16 * (ch ^ (row & (CPR - 1)))) = *reinterpret_cast<const uint4*>(y);
+                }
+            };
+            if constexpr (NQ == 1) {
+                collect(1.f);
+#pragma unroll
+                for (int cc = 0; cc < HD / 32 / HV; ++cc) put(half * (HD / 32 / HV) + cc, reinterpret_cast<const uint32_t*>(acc) + 32 * cc);
+            } else {
+#pragma unroll 1
+                for (int cc = 0; cc < HD / 32; ++cc) {
+                    uint32_t ov[32];
+                    tmem_ld32(t_o + 32 * cc, ov);
+                    tmem_ld_wait();
+                    put(cc, ov);
                 }
             }
             __syncwarp();
@@ -644,12 +671,12 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
             constexpr int i = i_(), buf = buf_(), st = st_();
             const uint32_t kd = desc_low(smem_u32(pr_raw) + (NQ * TERMS + st) * TILE, 1);
 #pragma unroll
-            for (int e = 0; e < TERMS; ++e) {
+            for (int e = TERMS - 1; e >= 0; --e) {  // the small parts first
                 const uint32_t qd = desc_low(smem_u32(pr_raw) + (i * TERMS + e) * TILE, 1);
 #pragma unroll
                 for (int kk = 0; kk < HD / 16; ++kk) {
                     const uint32_t off = ((kk >> 2) * ATOM_COL + 32 * (kk & 3)) >> 4;
-                    mma_ss<desc_high(1024), desc_high(1024)>(128 * buf, qd + off, kd + off, IDESC_S, (e > 0 || kk > 0) ? 1u : 0u, leader);
+                    mma_ss<desc_high(1024), desc_high(1024)>(128 * buf, qd + off, kd + off, IDESC_S, (e < TERMS - 1 || kk > 0) ? 1u : 0u, leader);
                 }
             }
             mma_commit(&sh.s_full[buf], leader);
@@ -658,11 +685,11 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
             constexpr int i = i_(), buf = buf_(), st = st_();
             const uint32_t vd = desc_low(smem_u32(pr_raw) + (NQ * TERMS + 2 + st) * TILE, 64);
 #pragma unroll
-            for (int e = 0; e < TERMS; ++e) {
+            for (int e = TERMS - 1; e >= 0; --e) {  // the small parts first
 #pragma unroll
                 for (int kk = 0; kk < PR_KT / 16; ++kk)
                     mma_ts<desc_high(NA * 1024)>(T_O + 128 * i, (e == 0 ? 128 * buf + (HV == 2 ? (kk >> 2) * 32 : 0) : T_LO + 64 * buf) + 8 * kk, vd + ((kk * 2 * (NA * 1024)) >> 4),
-                                                 IDESC_O, (e > 0 || kk > 0) ? 1u : acc, leader);
+                                                 IDESC_O, (e < TERMS - 1 || kk > 0) ? 1u : acc, leader);
             }
         };
         const std::integral_constant<int, 0> c0;
@@ -682,8 +709,8 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
                 ok = wait(&sh.v_full[n & 1], (n >> 1) & 1) && wait(&sh.p_full[n & 1], (n >> 1) & 1);
                 if (!ok) break;
                 fence_after();
-                if (n & 1) values(c0, c1, c1, 1u);
-                else values(c0, c0, c0, n > 0);
+                if (n & 1) values(c0, c1, c1, 0u);
+                else values(c0, c0, c0, 0u);
                 mma_commit(&sh.pv_done, leader);
                 mma_commit(&sh.v_empty[n & 1], leader);
             }

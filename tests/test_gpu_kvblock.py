@@ -501,3 +501,24 @@ def test_more_query_heads_than_a_tile_has_rows_are_refused(cuda):
     cache.reserve(0, 1)
     with pytest.raises(_lib.UnsupportedOperationException, match="128 query heads"):
         cache.attention(0, TokenBatch.of([0], [0], [1]), heads((1, 129, 64), 1, F16, cuda))
+
+
+@pytest.mark.parametrize("seqs,n", [(1, 130), (150, 1)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_float32_sums_stay_exact_over_long_caches(seqs, n, hd, cuda):
+    """The tensor cores truncate what they accumulate, some 2^-24 of the sum with each product. Pieces of at most 16
+    products added in FP32 are off by 16 2^-23 = 1.9e-6 at most, the scores (2^-20 each, independent) by less than 1e-6;
+    one chain over 12000 keys by 1e-5 and more."""
+    total = 12000
+    cache = new_cache(F32, seqs=seqs, heads_kv=1, hd=hd, block=64, blocks=190, per_seq=190)
+    k, v = heads((total, 1, hd), 98, F32, cuda), heads((total, 1, hd), 99, F32, cuda) + 0.5
+    cache.reserve(0, total)
+    cache.append(0, TokenBatch.of([0], [0], [total]), k, v)
+    cache.table[:] = cache.table[0].clone()  # every sequence reads the same pages
+    q = heads((n, 4, hd), 100, F32, cuda)
+    batch = TokenBatch.of(range(seqs), [total - n] * seqs, [n] * seqs)
+    y = f64(cache.attention(0, batch, q.repeat(seqs, 1, 1)))
+    want, _ = ref.attention(f64(q), ref.cache_values(f32(k), 64), ref.cache_values(f32(v), 64), total - n, hd ** -0.5)
+    for got in y.reshape(seqs, n, 4, hd):
+        assert np.linalg.norm(got - want) <= 3e-6 * np.linalg.norm(want), np.linalg.norm(got - want) / np.linalg.norm(want)
+    cache.check()
