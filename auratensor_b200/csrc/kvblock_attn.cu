@@ -591,7 +591,7 @@ StepPlan step_plan(const at_ctx* ctx, const KvbDev& c, const KvbBatch& b, int64_
     s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, (units + ST_WARPS - 1) / ST_WARPS));
     // Up to 8 splits that fit the GPU at once are one thread-block cluster (of
     // 2, 4 or 8 CTAs) and need neither workspace nor a second launch (one
-    // sequence of 513 tokens: 10.4 -> 7.3 us). In several waves a cluster's
+    // sequence of 513 tokens: 3.1 us less). In several waves a cluster's
     // CTAs hold their places until the last is done (64 sequences: 163 us
     // against 149 with the join as a kernel).
     const int pow2 = s.splits <= 2 ? s.splits : s.splits <= 4 ? 4 : 8;
