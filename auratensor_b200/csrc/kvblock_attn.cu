@@ -633,7 +633,9 @@ void launch_step(const StepParams& p, const StepPlan& s, cudaStream_t st) {
 constexpr int STEP_MAX_ROWS = 64;
 
 // The step kernel serves every sequence of at most STEP_MAX_ROWS query rows
-// per KV head; it is left out when the host's sizes say that there is none.
+// per KV head. The host's sizes are upper bounds, so a run may always be
+// shorter than they say; where they leave no room for it (equal prompts) the
+// step kernel is left out, and the prompt kernel takes every sequence.
 bool uses_step(const KvbBatch& b, int G) {
     return (int64_t)b.max_tokens * G <= STEP_MAX_ROWS || (int64_t)b.n_seqs * b.max_tokens > b.n_tokens;
 }
@@ -678,7 +680,8 @@ int at_kvb_attention(at_ctx* ctx, const at_kvb* cache, const at_token_batch* bat
         AT_REQUIRE(((uintptr_t)out & 15) == 0 && ((uintptr_t)q & (kvb_elem_bytes(dtype) - 1)) == 0, AT_ERR_INVALID_ARG,
                    "out must be 16-byte aligned, q aligned to its elements");
         AT_CUDA(cudaSetDevice(ctx->device));
-        if (uses_step(b, n_heads / c.hkv)) {
+        const bool step = uses_step(b, n_heads / c.hkv);
+        if (step) {
             const StepPlan s = step_plan(ctx, c, b, batch->max_end, n_heads, window, STEP_MAX_ROWS);
             AT_REQUIRE(workspace_bytes >= s.bytes && (s.bytes == 0 || (workspace && ((uintptr_t)workspace & 15) == 0)), AT_ERR_INVALID_ARG,
                        "attention: the workspace must be 16-byte aligned and hold at_kvb_attention_workspace bytes");
@@ -692,7 +695,8 @@ int at_kvb_attention(at_ctx* ctx, const at_kvb* cache, const at_token_batch* bat
             });
         }
         if ((int64_t)b.max_tokens * (n_heads / c.hkv) > STEP_MAX_ROWS)
-            launch_kvb_attn_prompt(c, b, dtype, n_heads, q, q_token_stride, q_head_stride, out, scale, window, STEP_MAX_ROWS, ctx->stream);
+            launch_kvb_attn_prompt(c, b, dtype, n_heads, q, q_token_stride, q_head_stride, out, scale, window, step ? STEP_MAX_ROWS : 0,
+                                   ctx->stream);
     });
 }
 

@@ -1,0 +1,47 @@
+"""The block cache where a call is at, or past, the edge of what it may ask for: sizes that are only upper bounds,
+positions without pages, rewinds, values of extreme scales. Tolerances are those of test_gpu_kvblock.py."""
+import numpy as np
+import pytest
+import torch
+
+import kvblock_ref as ref
+from auratensor_b200 import _lib
+from auratensor_b200.kvblock import TokenBatch
+from test_gpu_kvblock import BF16, F16, F32, ROUND, check_values, f32, f64, heads, new_cache
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- the host's sizes as upper bounds
+def loose(batch, nTokens, maxTokens, maxEnd):
+    return TokenBatch(batch.slots, batch.starts, batch.offsets, nTokens, maxTokens, maxEnd)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("counts,n_tokens,max_tokens", [((3,), 64, 64), ((10,), 512, 512), ((16,), 17, 17), ((1, 40, 16, 0), 160, 40),
+                                                        ((1, 2), 400, 200), ((5, 130), 260, 130), ((1, 1), 9, 3)])
+def test_sizes_may_be_upper_bounds(counts, n_tokens, max_tokens, dtype, cuda):
+    """What a captured graph has: the sizes of the launch are the largest, the runs on the device are shorter."""
+    seqs, group, prefix, total = len(counts), 4, 50, sum(counts)
+    cache = new_cache(dtype, seqs=seqs, hd=64, block=32, blocks=60, per_seq=12)
+    k, v = heads((seqs, 400, 2, 64), 101, dtype, cuda), heads((seqs, 400, 2, 64), 102, dtype, cuda)
+    for s in range(seqs):
+        cache.reserve(s, prefix + counts[s])
+        cache.append(0, TokenBatch.of([s], [0], [prefix]), k[s, :prefix], v[s, :prefix])
+    batch = loose(TokenBatch.of(range(seqs), [prefix] * seqs, counts), n_tokens, max_tokens, 12 * 32)
+    pad = torch.zeros((n_tokens - total, 2, 64), dtype=dtype, device=cuda)
+    new = [torch.cat([x[s, prefix:prefix + n] for s, n in enumerate(counts)] + [pad]) for x in (k, v)]
+    cache.append(0, batch, *new)
+    q = heads((n_tokens, 2 * group, 64), 103, dtype, cuda)
+    y = cache.attention(0, batch, q, out=torch.full_like(q, float("nan")))
+    gk, gv = cache.read(0, batch, F32)
+    cache.check()
+    y, qd, at = f64(y), f64(q), 0
+    for s, n in enumerate(counts):
+        check_values(cache, 0, s, k[s, :prefix + n], v[s, :prefix + n])
+        kd, vd = (ref.cache_values(f32(x[s, :prefix + n]), 32) for x in (k, v))
+        assert np.array_equal(f32(gk)[at:at + n], kd[prefix:].astype(np.float32)) and np.array_equal(f32(gv)[at:at + n], vd[prefix:].astype(np.float32))
+        want, mag = ref.attention(qd[at:at + n], kd, vd, prefix, 0.125)
+        tol = 5e-5 * mag + ROUND[dtype] * np.abs(want) + (0 if dtype == F32 else 2.0 ** -11 * mag)
+        assert np.all(np.abs(y[at:at + n] - want) <= tol), s
+        at += n
