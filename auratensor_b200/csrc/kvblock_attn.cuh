@@ -37,12 +37,18 @@ __device__ __forceinline__ float row_scale(float top) {
 
 // log2 d_v of a block as the attention kernels use it: weights are kept as
 // 2^(s + lv), their sum as 2^(s + lv) iv. A zero scale holds zeros only, so any
-// weight will do for its values. EXACT splits d_v into a power of two (lv, iv)
-// and a mantissa mv that multiplies the weights; else lv is the whole
-// logarithm (its error, 2^-20 at most, is far below 16-bit outputs) and mv 1.
+// weight will do for its values: it counts as 2^-80, far below the scales that
+// stand next to it, and 2^31 keys of the largest weight, 2^14, still sum to
+// less than FP32's end. The bounds of this form: a sum of n such weights over
+// blocks of scale d overflows at n 2^14 / d = 2^128 (2^17 keys: all visible
+// scales below 2^-97), and what lies 2^-134 below the largest t is lost, so
+// that scales up to 2^110 apart leave the sum its 24 bits.
+// EXACT splits d_v into a power of two (lv, iv) and a mantissa mv that
+// multiplies the weights; else lv is the whole logarithm (its error, 2^-20 at
+// most, is far below 16-bit outputs) and mv 1.
 template <bool EXACT>
 __device__ __forceinline__ void value_scale(float dv, float* lv, float* iv, float* mv) {
-    const float d = dv == 0.f ? 0x1p-100f : dv;
+    const float d = dv == 0.f ? 0x1p-80f : dv;
     if constexpr (EXACT) {
         const uint32_t u = __float_as_uint(d);
         const int e = (int)(u >> 23) - 127;  // d is normal, or NaN

@@ -22,7 +22,8 @@
 // Arithmetic, per row, in log2 units: t_j = s_j + log2 d_v(j), P_j = 2^(t_j - r)
 // with a reference r that follows the row's largest t; out = sum P_j v8_j /
 // sum P_j / d_v(j). The values' scale is part of the exponent, so P fills
-// f16's range whatever the blocks' scales are, and costs no product; FP32
+// f16's range whatever the blocks' scales are (value_scale says how far apart
+// they may lie), and costs no product; FP32
 // queries keep log2 d_v to its integer part and multiply by the mantissa, as
 // its logarithm is not exact. r is set 2^8 below the row's maximum, and moved
 // (with O, in TMEM, rescaled) only when the maximum outgrows it by 2^14, which

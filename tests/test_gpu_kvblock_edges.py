@@ -45,3 +45,26 @@ def test_sizes_may_be_upper_bounds(counts, n_tokens, max_tokens, dtype, cuda):
         tol = 5e-5 * mag + ROUND[dtype] * np.abs(want) + (0 if dtype == F32 else 2.0 ** -11 * mag)
         assert np.all(np.abs(y[at:at + n] - want) <= tol), s
         at += n
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_many_keys_without_values(dtype, cuda):
+    """38000 keys whose values are all zero, then 1000 that have some: the zeros' weights count in full."""
+    total, empty, n = 39000, 38000, 130
+    cache = new_cache(dtype, seqs=1, heads_kv=1, hd=64, block=128, blocks=310, per_seq=310)
+    k, v = heads((total, 1, 64), 121, F32, cuda) * 0.1, heads((total, 1, 64), 122, F32, cuda) + 1
+    v[:empty] = 0
+    k[:, 0, 0] = 1
+    k[128:, 0, 0] = 1 + 4.1  # after the first tile the scores are 4.1 higher (in powers of e), 5.9 in powers of 2
+    k, v = k.to(dtype), v.to(dtype)
+    q = heads((n, 2, 64), 123, F32, cuda) * 0.01
+    q[:, :, 0] = 8.0
+    q = q.to(dtype)
+    cache.reserve(0, total)
+    cache.append(0, TokenBatch.of([0], [0], [total]), k, v)
+    y = f64(cache.attention(0, TokenBatch.of([0], [total - n], [n]), q))
+    want, mag = ref.attention(f64(q), ref.cache_values(f32(k), 128), ref.cache_values(f32(v), 128), total - n, 0.125)
+    # a chain of 39000 keys in 16 bits: 128-key pieces, each off by 2^-23 of the sum
+    tol = (5e-5 + (0 if dtype == F32 else 2.0 ** -11 + 39000 / 16 * 2.0 ** -23)) * mag + ROUND[dtype] * np.abs(want)
+    assert np.all(np.abs(y - want) <= tol), float((np.abs(y - want) / tol).max())
+    cache.check()
