@@ -14,6 +14,7 @@
 // error builds up. Two blocks, so that the next append may also start
 // anywhere in the last block written or the one before it (a rejected draft
 // is overwritten).
+#include <algorithm>
 #include <cstdint>
 #include <string>
 
@@ -63,7 +64,9 @@ KvbBatch kvb_batch(const at_kvb* c, const at_token_batch* b) {
     AT_REQUIRE(b->max_end <= (int64_t)c->max_blocks * c->block_tokens, AT_ERR_STATE,
                "position " + std::to_string(b->max_end) + " is past the cache's " +
                    std::to_string((int64_t)c->max_blocks * c->block_tokens) + " positions per sequence");
-    return KvbBatch{b->n_seqs, b->n_tokens, b->max_tokens, b->slots, b->starts, b->offsets};
+    // a run is no longer than a sequence's positions, whatever the host's bound
+    const int most = (int)std::min<int64_t>(b->max_tokens, (int64_t)c->max_blocks * c->block_tokens);
+    return KvbBatch{b->n_seqs, b->n_tokens, most, b->slots, b->starts, b->offsets};
 }
 
 namespace {
@@ -302,10 +305,10 @@ __global__ void __launch_bounds__(READ_THREADS) kvb_read_kernel(KvbDev c, KvbBat
 template <class T, int HD>
 void launch_append(const KvbDev& c, const KvbBatch& b, const AppendSrc<T>& k, const AppendSrc<T>& v, cudaStream_t s) {
     const int B = 1 << c.lb;
-    const int touched = (b.max_tokens + B - 2) / B + 1;
+    const int touched = (int)(((int64_t)b.max_tokens + B - 2) / B) + 1;
     AT_REQUIRE((int64_t)b.n_seqs * touched <= INT32_MAX && c.hkv <= 32767, AT_ERR_INVALID_ARG, "the batch is too large for one append");
     const dim3 grid(b.n_seqs * touched, 2 * c.hkv);
-    const int few = b.max_tokens * (HD / 8);  // chunks of a sequence's new rows in one block at most
+    const int few = std::min(b.max_tokens, B) * (HD / 8);  // chunks of a sequence's new rows in one block at most
     if (few <= 32) kvb_append_kernel<T, HD, 32, 1><<<grid, 32, 0, s>>>(c, b, k, v, touched);
     else if (few <= 128) kvb_append_kernel<T, HD, 32, 4><<<grid, 32, 0, s>>>(c, b, k, v, touched);
     else {
@@ -360,7 +363,7 @@ int at_kvb_read(at_ctx* ctx, const at_kvb* cache, const at_token_batch* batch, i
         if (b.n_seqs == 0 || b.max_tokens == 0) return;
         AT_REQUIRE(k_out || v_out, AT_ERR_INVALID_ARG, "null outputs");
         AT_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, AT_ERR_INVALID_ARG, "outputs must be 16-byte aligned");
-        const int chunks = (b.max_tokens + READ_TOKENS - 1) / READ_TOKENS;
+        const int chunks = (int)(((int64_t)b.max_tokens + READ_TOKENS - 1) / READ_TOKENS);
         AT_REQUIRE((int64_t)b.n_seqs * chunks <= INT32_MAX && c.hkv <= 32767, AT_ERR_INVALID_ARG, "the batch is too large for one read");
         const dim3 grid(b.n_seqs * chunks, c.hkv * (k_out && v_out ? 2 : 1));
         AT_CUDA(cudaSetDevice(ctx->device));

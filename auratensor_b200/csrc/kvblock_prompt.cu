@@ -762,7 +762,7 @@ void prompt_launch(PromptParams p, cudaStream_t s) {
     }();
     AT_REQUIRE(regs == pr_launch_regs<T>(), AT_ERR_CUDA, "prompt attention was built with another register count than its warpgroups share");
     const int per = pr_tiles<T>() * (PR_ROWS / p.G);
-    p.blocks = (p.b.max_tokens + per - 1) / per;
+    p.blocks = (int)(((int64_t)p.b.max_tokens + per - 1) / per);
     const int64_t grid = (int64_t)p.blocks * p.c.hkv * p.b.n_seqs;
     AT_REQUIRE(grid <= INT32_MAX, AT_ERR_INVALID_ARG, "the batch is too large for one call");
     kern<<<(int)grid, pr_threads<T>(), pr_smem<T, HD>(), s>>>(p);

@@ -68,3 +68,15 @@ def test_many_keys_without_values(dtype, cuda):
     tol = (5e-5 + (0 if dtype == F32 else 2.0 ** -11 + 39000 / 16 * 2.0 ** -23)) * mag + ROUND[dtype] * np.abs(want)
     assert np.all(np.abs(y - want) <= tol), float((np.abs(y - want) / tol).max())
     cache.check()
+
+
+def test_a_bound_of_many_tokens_is_not_cut_to_32_bits(cuda):
+    """2^27 tokens of 16 chunks each are 2^31 chunks."""
+    bound, n = 1 << 27, 100
+    cache = new_cache(F16, seqs=1, hd=128, block=128, blocks=4, per_seq=4)
+    cache.reserve(0, n)
+    row = heads((1, 2, 128), 111, F16, cuda)
+    batch = loose(TokenBatch.of([0], [0], [n]), bound, bound, 512)
+    cache.append(0, batch, row.expand(bound, 2, 128), row.expand(bound, 2, 128))
+    cache.check()
+    check_values(cache, 0, 0, row.expand(n, 2, 128), row.expand(n, 2, 128))
