@@ -28,6 +28,7 @@ from . import _lib
 from ._lib import GGML_BF16, GGML_F16, GGML_F32, IllegalArgumentException, IllegalStateException, KvBlocksC, TokenBatchC, lib
 from .core import _current_stream, context
 
+NO_PAGE = -1  # table entry of a position that was not reserved: outside the pool, so that the kernels report it
 DTYPE_CODES = {torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16}
 
 
@@ -156,7 +157,7 @@ class BlockKvCache:
         blocks, scales = (layers, nBlocks, headCountKv, blockTokens, headDim), (layers, nBlocks, headCountKv)
         ring = (layers, maxSeqs, headCountKv, 2 * blockTokens)
         self = cls(zeros(*blocks, dt=torch.int8), zeros(*blocks, dt=torch.int8), zeros(*scales), zeros(*scales),
-                   zeros(maxSeqs, maxBlocks, dt=torch.int32), zeros(*ring, headDim, dt=dtype), zeros(*ring, headDim, dt=dtype),
+                   torch.full((maxSeqs, maxBlocks), NO_PAGE, dtype=torch.int32, device=dev), zeros(*ring, headDim, dt=dtype), zeros(*ring, headDim, dt=dtype),
                    zeros(*ring), zeros(*ring), dtype, zeros(1, dt=torch.int32))
         self._free = list(range(nBlocks - 1, -1, -1))
         self._pages = [[] for _ in range(maxSeqs)]
@@ -177,7 +178,9 @@ class BlockKvCache:
             raise IllegalStateException(_lib.AT_ERR_STATE, "the page table of a wrapped cache is the caller's")
 
     def reserve(self, slot: int, length: int) -> None:
-        """Gives slot the pages of its first `length` positions."""
+        """Gives slot the pages of its first `length` positions. Calls on
+        positions without a page write nothing, read NaN, and make ``check``
+        raise."""
         self._own_pages()
         if not 0 <= slot < self.maxSeqs:
             _bad(f"slot {slot} out of range [0, {self.maxSeqs})")
@@ -199,8 +202,11 @@ class BlockKvCache:
         self._own_pages()
         if not 0 <= slot < self.maxSeqs:
             _bad(f"slot {slot} out of range [0, {self.maxSeqs})")
-        self._free.extend(reversed(self._pages[slot]))
-        self._pages[slot] = []
+        pages = self._pages[slot]
+        if pages:
+            self.table[slot, :len(pages)] = NO_PAGE
+            self._free.extend(reversed(pages))
+            self._pages[slot] = []
 
     def freeBlocks(self) -> int:
         self._own_pages()

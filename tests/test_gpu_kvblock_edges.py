@@ -80,3 +80,37 @@ def test_a_bound_of_many_tokens_is_not_cut_to_32_bits(cuda):
     cache.append(0, batch, row.expand(bound, 2, 128), row.expand(bound, 2, 128))
     cache.check()
     check_values(cache, 0, 0, row.expand(n, 2, 128), row.expand(n, 2, 128))
+
+
+# ---------------------------------------------------------------- positions without a page
+def test_positions_that_were_not_reserved_have_no_page(cuda):
+    cache = new_cache(F32, seqs=3, hd=64, block=32)
+    k, v = heads((40, 2, 64), 151, F32, cuda), heads((40, 2, 64), 152, F32, cuda)
+    other, q = heads((40, 2, 64), 153, F32, cuda), heads((1, 4, 64), 154, F32, cuda)
+    cache.reserve(0, 40)
+    cache.append(0, TokenBatch.of([0], [0], [40]), k, v)
+    cache.check()
+
+    def refused(call):
+        r = call()
+        with pytest.raises(_lib.IllegalStateException, match="outside the pool"):
+            cache.check()
+        check_values(cache, 0, 0, k, v)
+        return r
+
+    refused(lambda: cache.append(0, TokenBatch.of([1], [0], [40]), other, other))   # nothing reserved
+    cache.reserve(1, 10)
+    refused(lambda: cache.append(0, TokenBatch.of([1], [20], [40]), other, other))  # past what was
+    assert torch.isnan(refused(lambda: cache.read(0, TokenBatch.of([2], [0], [5])))[0]).all()
+    assert torch.isnan(refused(lambda: cache.attention(0, TokenBatch.of([2], [0], [1]), q))).all()
+    # a released slot's pages may be another's by now
+    cache.release(1)
+    cache.reserve(2, 40)
+    cache.append(0, TokenBatch.of([2], [0], [40]), other, other)
+    cache.check()
+    refused(lambda: cache.append(0, TokenBatch.of([1], [0], [10]), k[:10], k[:10]))
+    check_values(cache, 0, 2, other, other)
+    cache.reserve(1, 10)  # reserved anew it is usable
+    cache.append(0, TokenBatch.of([1], [0], [10]), other[:10], k[:10])
+    cache.check()
+    check_values(cache, 0, 1, other[:10], k[:10])
