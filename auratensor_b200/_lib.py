@@ -98,7 +98,7 @@ class TokenBatchC(C.Structure):
                 ("max_end", C.c_int64), ("slots", C.c_void_p), ("starts", C.c_void_p), ("offsets", C.c_void_p)]
 
 
-KVB_BAD_SEQ, KVB_BAD_BLOCK, KVB_STALLED = 1, 2, 4
+KVB_BAD_SEQ, KVB_BAD_BLOCK, KVB_STALLED, KVB_STALE_TAIL = 1, 2, 4, 8
 
 _vp, _i, _i64, _sz, _f = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_float
 _PP = C.POINTER(C.c_void_p)

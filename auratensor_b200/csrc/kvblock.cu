@@ -13,7 +13,10 @@
 // holds depends on its tokens alone, not on how appends cut them, and no
 // error builds up. Two blocks, so that the next append may also start
 // anywhere in the last block written or the one before it (a rejected draft
-// is overwritten).
+// is overwritten). The ring holds, of the even and of the odd blocks, the one
+// written last: an append that starts inside another block would take that
+// one's rows for its own, so the row before its first is compared with what
+// the page holds of it, and where they differ the append is reported instead.
 #include <algorithm>
 #include <cstdint>
 #include <string>
@@ -111,18 +114,32 @@ __device__ __forceinline__ uint32_t max_bits_f32(uint32_t m) {
     }
 }
 
-// Eight quants. 1.5 2^23 + x rounds x to the nearest integer (ties to even) in
+// A quant in the low byte, and eight. 1.5 2^23 + x rounds x to the nearest integer (ties to even) in
 // the low bits of the sum: its low byte is q in two's complement (one addition
 // instead of a conversion, which runs at an eighth of its rate).
+__device__ __forceinline__ uint32_t quant1(float x, float inv) { return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.f)); }
 __device__ __forceinline__ uint2 quant8(const float* x, float inv) {
     uint32_t b[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], inv), 12582912.f));
+    for (int i = 0; i < 8; ++i) b[i] = quant1(x[i], inv);
     uint32_t w[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
         w[i] = __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x0040), __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040), 0x5410);
     return make_uint2(w[0], w[1]);
+}
+
+// Whether a row of the ring is what its row of the page was quantized from
+// (warp-uniform). A poisoned block, whose scale is NaN, cannot be told.
+template <class T, int HD>
+__device__ __forceinline__ bool tail_intact(const int8_t* page_row, const T* tail_row, float row_max, float held) {
+    constexpr int E = HD / 32;  // elements per lane
+    const int col = E * (threadIdx.x & 31);
+    const float inv = held > 0.f ? __fdiv_rn(1.f, held) : 0.f, d = __fdiv_rn(row_max, 127.f);
+    bool differs = !((d < 0x1p-126f ? 0.f : d) <= held);
+#pragma unroll
+    for (int i = 0; i < E; ++i) differs |= (int8_t)quant1(to_f32<T>(tail_row[col + i]), inv) != page_row[col + i];
+    return held != held || !__any_sync(0xffffffffu, differs);
 }
 
 template <class T>
@@ -137,10 +154,12 @@ struct AppendSrc {
 // between the maximum and the quantization, so every value is read once. NT
 // threads: 256 for whole blocks, one warp (its barriers wait for no other) for
 // a few tokens. 8 BF16 prompts up to 8191 tokens, 8 heads of 128, written and
-// read back: 119 us, 5.3 TB/s over both kernels; the write is bound by its
+// read back: 120 us, 5.2 TB/s over both kernels; the write is bound by its
 // instructions (packed maxima, products and roundings fill 86 % of the issue
 // slots), not by memory. K and V of a block in one CTA spill: 125 us. One token
-// of one sequence, written and read back: 4.6 us.
+// of one sequence, written and read back: 4.9 us, 0.4 of it the look at the
+// tail (held in eight values per lane that look took 57 registers for 48, a
+// CTA per SM, and 5 us of the prompts; a row spread over the warp takes none).
 template <class T, int HD, int NT, int NCH>
 __global__ void __launch_bounds__(NT) kvb_append_kernel(KvbDev c, KvbBatch b, AppendSrc<T> sk, AppendSrc<T> sv, int max_touched) {
     constexpr int CPR = HD / 8;  // chunks per row: a row's chunks are neighbouring lanes
@@ -178,6 +197,15 @@ __global__ void __launch_bounds__(NT) kvb_append_kernel(KvbDev c, KvbBatch b, Ap
     float* tail_max = (is_v ? c.vtm : c.ktm) + ring0;
     const int last = (end - 1) >> c.lb;
     const int ring_mask = 2 * B - 1;
+    // An append inside a block needs the block's older rows in the ring. Every
+    // warp looks for itself, before the CTA writes anything: all leave together.
+    if (lo > base) {
+        const int p = (lo - 1) & ring_mask;
+        if (!tail_intact<T, HD>(dst + (size_t)(lo - 1 - base) * HD, tail + (size_t)p * HD, tail_max[p], held)) {
+            if (tid == 0) kvb_flag(c.status, KVB_STALE_TAIL);
+            return;
+        }
+    }
     // The rows of blocks last - 1 and last go to the ring. If this append
     // begins inside a block and another block of the same parity is kept, the
     // ring rows that the first block still reads are the ones that block

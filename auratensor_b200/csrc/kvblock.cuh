@@ -17,6 +17,7 @@ namespace at {
 constexpr int KVB_BAD_SEQ = 1;    // a slot, start or offset outside its range: the sequence was skipped
 constexpr int KVB_STALLED = 4;    // a bounded wait inside a kernel ran out: its output is not valid
 constexpr int KVB_BAD_BLOCK = 2;  // a block-table entry outside the pool: reads give NaN, writes are dropped
+constexpr int KVB_STALE_TAIL = 8;  // an append inside a block whose older rows the tail no longer has: that block was not written
 
 struct KvbDev {
     int hkv, hd, lb;  // lb: log2(block_tokens)

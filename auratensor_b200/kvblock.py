@@ -235,7 +235,10 @@ class BlockKvCache:
 
     def append(self, layer: int, batch: TokenBatch, k: torch.Tensor, v: torch.Tensor) -> None:
         """Quantizes the batch's K and V ([tokens][kv heads][head dim], the
-        cache's dtype; token and head strides are free) into the cache."""
+        cache's dtype; token and head strides are free) into the cache. A run
+        starts at its slot's next position or goes back: to the first row of
+        any block, or inside the last block written or the one before it, but
+        not further for having gone back before (``check`` reports it)."""
         ref = self._layer(layer)
         shape, ks, vs = (batch.nTokens, self.headCountKv, self.headDim), k.stride(), v.stride()
         for t, s, name in ((k, ks, "k"), (v, vs, "v")):
@@ -294,8 +297,9 @@ class BlockKvCache:
         return out
 
     def check(self) -> None:
-        """Raises when a kernel met a slot, position or page outside its range
-        since the last check (waits for the device)."""
+        """Raises when a kernel met a slot, position or page outside its range,
+        or an append that it could not make, since the last check (waits for
+        the device). A cache wrapped without a status tensor cannot tell."""
         if self.status is None:
             return
         bits = int(self.status.item())
@@ -304,4 +308,6 @@ class BlockKvCache:
             raise IllegalStateException(_lib.AT_ERR_STATE, "block KV cache: " + " and ".join(
                 m for b, m in ((_lib.KVB_BAD_SEQ, "a slot, start or offset out of range (its sequence was skipped)"),
                                (_lib.KVB_STALLED, "a wait inside a kernel that ran out (its output is not valid)"),
-                               (_lib.KVB_BAD_BLOCK, "a page outside the pool (writes dropped, reads NaN)")) if bits & b))
+                               (_lib.KVB_BAD_BLOCK, "a page outside the pool (writes dropped, reads NaN)"),
+                               (_lib.KVB_STALE_TAIL, "an append inside a block whose older rows the tail no longer has (not written there)"))
+                if bits & b))

@@ -365,7 +365,8 @@ int at_sample(float* logits, int vocab, const int* history, int n_history, float
  * (row p % (2 block_tokens)) with each row's max|x|: when a new token raises
  * an open block's maximum, its older rows are quantized again from them, so a
  * block's contents depend on its tokens alone, not on how appends cut them.
- * Pages that are full are never written again and may be shared by slots. */
+ * Slots may share pages that are full, as long as no append goes back into
+ * them: it would change the page for all of them. */
 typedef struct at_kvb {
     int32_t dtype;                 /* type of appended K/V and of the tail: AT_GGML_F32, _F16, _BF16 */
     int32_t n_kv_heads;
@@ -384,11 +385,12 @@ typedef struct at_kvb {
     float* k_tail_max;             /* [max_seqs][n_kv_heads][2 block_tokens] */
     float* v_tail_max;
     const int32_t* block_table;    /* [max_seqs][max_blocks] */
-    int32_t* status;               /* one word or NULL: AT_KVB_BAD_* bits are set when a kernel meets them */
+    int32_t* status;               /* one word or NULL: AT_KVB_* bits are set when a kernel meets them */
 } at_kvb;
 #define AT_KVB_BAD_SEQ   1         /* slot, start or offset out of range: that sequence was skipped */
 #define AT_KVB_BAD_BLOCK 2         /* block_table entry outside the pool: writes dropped, reads NaN */
 #define AT_KVB_STALLED   4         /* a bounded wait inside a kernel ran out: its output is not valid */
+#define AT_KVB_STALE_TAIL 8        /* an append inside a block whose older rows the tail no longer has: not written there */
 /* Runs of consecutive tokens, one per sequence, packed one after the other:
  * sequence s has slot slots[s] and the tokens offsets[s] .. offsets[s+1] of the
  * packed arrays, at positions starts[s], starts[s] + 1, ... The arrays are on
@@ -406,9 +408,13 @@ typedef struct at_token_batch {
 } at_token_batch;
 /* Writes the batch's K and V ([n_tokens][n_kv_heads][head_dim] of the cache's
  * dtype, head_dim contiguous, strides in elements; the KVCache.append of this
- * cache, inference/KVCache.java:79-95). A run may start anywhere from the
- * first position of the block before the slot's last written one: what lies
- * after it is overwritten. Runs on the context's stream. */
+ * cache, inference/KVCache.java:79-95). A run may start at the slot's next
+ * position, at the first row of any block, or inside a block whose rows the
+ * tail still has (of the even and of the odd blocks, the one written last: the
+ * two last blocks, until an earlier one is written again); what lies after it
+ * is overwritten. Inside any other block it cannot quantize the older rows
+ * again: AT_KVB_STALE_TAIL is set and that block is left as it was. Runs on
+ * the context's stream. */
 int at_kvb_append(at_ctx* ctx, const at_kvb* cache, const at_token_batch* batch, const void* k, int64_t k_token_stride,
                   int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride);
 /* Reads the batch's positions back as values, [n_tokens][n_kv_heads][head_dim]

@@ -114,3 +114,39 @@ def test_positions_that_were_not_reserved_have_no_page(cuda):
     cache.append(0, TokenBatch.of([1], [0], [10]), other[:10], k[:10])
     cache.check()
     check_values(cache, 0, 1, other[:10], k[:10])
+
+
+# ---------------------------------------------------------------- rewinding
+def test_a_second_rewind_behind_the_kept_rows_is_reported(cuda):
+    """0..99 in blocks of 32 keeps the originals of blocks 2 and 3. After a rewind into block 2 those of block 1 are
+    still gone: an append inside it cannot quantize its older rows again and must not take block 3's for them."""
+    cache = new_cache(F32, hd=64, block=32)
+    k, v = heads((100, 2, 64), 131, F32, cuda) * 4, heads((100, 2, 64), 132, F32, cuda)
+    small = heads((9, 2, 64), 133, F32, cuda)
+    cache.reserve(0, 200)
+    cache.append(0, TokenBatch.of([0], [0], [100]), k, v)
+    cache.append(0, TokenBatch.of([0], [70], [9]), small, small)
+    cache.check()
+    page = int(cache.table[0, 1])
+    before = [x[0, page].clone() for x in (cache.kBlocks, cache.vBlocks, cache.kScales, cache.vScales)]
+    cache.append(0, TokenBatch.of([0], [40], [5]), small[:5], small[:5])
+    with pytest.raises(_lib.IllegalStateException, match="older rows"):
+        cache.check()
+    for a, x in zip(before, (cache.kBlocks, cache.vBlocks, cache.kScales, cache.vScales)):
+        assert torch.equal(a, x[0, page])
+    check_values(cache, 0, 0, torch.cat([k[:70], small]), torch.cat([v[:70], small]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_repeated_rewinds_within_the_kept_rows(dtype, cuda):
+    """Inside a block whose originals are still kept, and at the first row of any block, as often as one likes."""
+    cache = new_cache(dtype, hd=64, block=32)
+    held_k, held_v = [heads((0, 2, 64), 1, dtype, cuda) for _ in range(2)]
+    cache.reserve(0, 200)
+    for i, (at, c) in enumerate(((0, 100), (70, 9), (65, 3), (68, 40), (97, 2), (66, 1), (32, 50), (60, 4), (0, 33), (5, 1))):
+        scale = 4.0 if i % 2 == 0 else 0.25
+        k, v = heads((c, 2, 64), 140 + 2 * i, dtype, cuda) * scale, heads((c, 2, 64), 141 + 2 * i, dtype, cuda) * scale
+        cache.append(0, TokenBatch.of([0], [at], [c]), k, v)
+        cache.check()
+        held_k, held_v = torch.cat([held_k[:at], k]), torch.cat([held_v[:at], v])
+        check_values(cache, 0, 0, held_k, held_v)
