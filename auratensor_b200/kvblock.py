@@ -28,6 +28,7 @@ from . import _lib
 from ._lib import GGML_BF16, GGML_F16, GGML_F32, IllegalArgumentException, IllegalStateException, KvBlocksC, TokenBatchC, lib
 from .core import _current_stream, context
 
+INT32_MAX, INT64_MAX = (1 << 31) - 1, (1 << 63) - 1
 NO_PAGE = -1  # table entry of a position that was not reserved: outside the pool, so that the kernels report it
 DTYPE_CODES = {torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16}
 
@@ -60,6 +61,9 @@ class TokenBatch:
             _bad("batch tensors must be on a CUDA device")
         if not (slots.is_contiguous() and starts.is_contiguous() and offsets.is_contiguous()):
             _bad("batch tensors must be contiguous")
+        for name, x, most in (("nTokens", nTokens, INT32_MAX), ("maxTokens", maxTokens, INT32_MAX), ("maxEnd", maxEnd, INT64_MAX)):
+            if not 0 <= x <= most:
+                _bad(f"{name} must be in [0, {most}], got {x}")
         self.slots, self.starts, self.offsets = slots, starts, offsets
         self.nSeqs, self.nTokens, self.maxTokens, self.maxEnd = n, int(nTokens), int(maxTokens), int(maxEnd)
         self._c = TokenBatchC(n, self.nTokens, self.maxTokens, 0, self.maxEnd, slots.data_ptr(), starts.data_ptr(), offsets.data_ptr())
@@ -79,6 +83,8 @@ class TokenBatch:
         offsets = [0]
         for c in counts:
             offsets.append(offsets[-1] + c)
+        if max(slots, default=0) > INT32_MAX or offsets[-1] > INT32_MAX or any(s + c > INT64_MAX for s, c in zip(starts, counts)):
+            _bad("slots and the number of tokens must fit 32 bits, positions 64")
         dev = torch.device("cuda") if device is None else device
         flat = torch.tensor(starts + slots + offsets, dtype=torch.int64).to(dev)
         i32 = flat[n:].to(torch.int32)
@@ -282,7 +288,10 @@ class BlockKvCache:
         elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous():
             _bad("out must be contiguous and of q's type and shape")
         self._on_device(q, out, batch.slots)
-        heads, window = q.shape[1], int(window)
+        window = int(window)
+        if window < 0:
+            _bad("window must not be negative")
+        heads, window = q.shape[1], min(window, INT32_MAX)  # positions fit 31 bits: a longer window hides nothing either
         index, L = self.device.index, lib()
         ctx, need = context(index), C.c_size_t()
         rc = L.at_kvb_attention_workspace(ctx, ref, batch._ref, heads, window, C.byref(need))

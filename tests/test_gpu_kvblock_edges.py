@@ -150,3 +150,23 @@ def test_repeated_rewinds_within_the_kept_rows(dtype, cuda):
         cache.check()
         held_k, held_v = torch.cat([held_k[:at], k]), torch.cat([held_v[:at], v])
         check_values(cache, 0, 0, held_k, held_v)
+
+
+def test_windows_of_more_than_31_bits(cuda):
+    cache = new_cache(F32, hd=64, block=32)
+    k, q = heads((50, 2, 64), 161, F32, cuda), heads((1, 4, 64), 162, F32, cuda)
+    cache.reserve(0, 50)
+    cache.append(0, TokenBatch.of([0], [0], [50]), k, k)
+    batch = TokenBatch.of([0], [49], [1])
+    want = cache.attention(0, batch, q)
+    for window in ((1 << 32) + 5, 1 << 31, 1 << 40):
+        assert torch.equal(cache.attention(0, batch, q, window=window), want)
+    with pytest.raises(_lib.IllegalArgumentException):
+        cache.attention(0, batch, q, window=5 - (1 << 32))
+
+
+def test_sizes_that_do_not_fit_are_refused(cuda):
+    b = TokenBatch.of([0], [0], [3])
+    for sizes in (((1 << 32) + 3, 3, 3), (3, (1 << 32) + 3, 3), (-1, 3, 3), (3, -1, 3), (3, 3, 1 << 64), (3, 3, -1)):
+        with pytest.raises(_lib.IllegalArgumentException, match="must be in"):
+            loose(b, *sizes)
