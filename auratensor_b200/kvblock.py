@@ -59,6 +59,8 @@ class TokenBatch:
             _bad(f"{n} slots need {n} starts and {n + 1} offsets, got {starts.numel()} and {offsets.numel()}")
         if not (slots.is_cuda and starts.is_cuda and offsets.is_cuda):
             _bad("batch tensors must be on a CUDA device")
+        if not slots.get_device() == starts.get_device() == offsets.get_device():
+            _bad("batch tensors must be on one device")
         if not (slots.is_contiguous() and starts.is_contiguous() and offsets.is_contiguous()):
             _bad("batch tensors must be contiguous")
         for name, x, most in (("nTokens", nTokens, INT32_MAX), ("maxTokens", maxTokens, INT32_MAX), ("maxEnd", maxEnd, INT64_MAX)):
