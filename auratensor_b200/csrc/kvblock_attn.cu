@@ -653,10 +653,9 @@ int at_kvb_attention_workspace(at_ctx* ctx, const at_kvb* cache, const at_token_
     return guard([&] {
         AT_REQUIRE(ctx && cache && batch, AT_ERR_INVALID_ARG, "null argument");
         AT_REQUIRE(bytes, AT_ERR_INVALID_ARG, "null output");
-        AT_REQUIRE(n_heads > 0 && n_heads % cache->n_kv_heads == 0, AT_ERR_INVALID_ARG,
-                   "query heads must be a multiple of the KV heads");
         const KvbDev c = kvb_dev(ctx, cache, false);
         const KvbBatch b = kvb_batch(cache, batch);
+        AT_REQUIRE(n_heads > 0 && n_heads % c.hkv == 0, AT_ERR_INVALID_ARG, "query heads must be a multiple of the KV heads");
         *bytes = 0;
         if (b.n_seqs == 0 || b.max_tokens == 0) return;
         if (uses_step(b, n_heads / c.hkv)) *bytes = step_plan(ctx, c, b, batch->max_end, n_heads, window, STEP_MAX_ROWS).bytes;
