@@ -112,6 +112,7 @@ SIGNATURES = {
     "at_ctx_synchronize": [_vp],
     "at_ctx_stream": [_vp, _PP],
     "at_ctx_set_stream": [_vp, _vp],
+    "at_ctx_bind_stream": [_vp, _vp],
     "at_alloc": [_vp, _sz, _PP],
     "at_free": [_vp, _vp],
     "at_memcpy_h2d": [_vp, _vp, _vp, _sz],

@@ -34,7 +34,6 @@ _TORCH = {DType.FP32: torch.float32, DType.FP16: torch.float16, DType.INT8: torc
 
 _ctx_lock = threading.Lock()
 _ctxs: dict = {}
-_bound: dict = {}  # device -> the stream its context was last bound to
 
 
 def _current_stream(device: int) -> int:
@@ -46,7 +45,8 @@ _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream
 
 
 def context(device: int | None = None) -> int:
-    """The per-device at_ctx of this process, bound to torch's current stream."""
+    """The per-device at_ctx of this process, bound to torch's current stream
+    for the calling thread."""
     if device is None:
         device = torch.cuda.current_device()
     ctx = _ctxs.get(device)
@@ -57,10 +57,9 @@ def context(device: int | None = None) -> int:
                 p = C.c_void_p()
                 call("at_ctx_create", device, C.byref(p))
                 ctx = _ctxs[device] = p.value
-    stream = _current_stream(device)
-    if _bound.get(device) != stream:
-        call("at_ctx_set_stream", ctx, C.c_void_p(stream))
-        _bound[device] = stream
+    rc = _lib.lib().at_ctx_bind_stream(ctx, _current_stream(device))
+    if rc:
+        _lib.check(rc)
     return ctx
 
 

@@ -3,6 +3,7 @@
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstdint>
 #include <cstdio>
 #include <stdexcept>
@@ -52,11 +53,26 @@ int guard(F&& body) {
 
 struct NcclApi;  // dlopen'd NCCL entry points
 
+// The stream of a context: what the calling thread bound it to, or, in a
+// thread that bound none, what the context was given last. Two threads that
+// work on streams of their own then cannot move one another's launches.
+class CtxStream {
+  public:
+    operator cudaStream_t() const;
+    void set(cudaStream_t s);   // for all threads without a binding, this one's is dropped
+    void bind(cudaStream_t s);  // for this thread, and for those without a binding
+
+  private:
+    static uint64_t next_id();
+    const uint64_t id_ = next_id();  // never used twice: a later context at this address has no old bindings
+    std::atomic<cudaStream_t> last_{nullptr};
+};
+
 }  // namespace at
 
 struct at_ctx {
     int device = 0;
-    cudaStream_t stream = nullptr;      // stream every launch of this context uses
+    at::CtxStream stream;               // stream every launch of this context uses
     cudaStream_t own_stream = nullptr;  // stream created with the context
     int num_sms = 148;
     // tensor parallelism

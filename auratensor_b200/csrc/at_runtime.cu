@@ -1,8 +1,11 @@
 // Runtime, memory, block codecs, planar re-layout and the core.Kernels ops of
 // libauratensor_cuda.so.
+#include <algorithm>
 #include <cstring>
 #include <mutex>
 #include <string>
+#include <utility>
+#include <vector>
 
 #include "at_internal.h"
 #include "dev_common.cuh"
@@ -11,6 +14,7 @@ namespace at {
 
 namespace {
 thread_local std::string g_last_error;
+thread_local std::vector<std::pair<uint64_t, cudaStream_t>> g_bound;  // this thread's contexts (CtxStream ids) and their streams
 constexpr int TPB = 256;
 
 inline int grid_for(int64_t n, int tpb = TPB) {
@@ -21,6 +25,29 @@ inline int grid_for(int64_t n, int tpb = TPB) {
 }  // namespace
 
 void set_last_error(const std::string& msg) { g_last_error = msg; }
+
+CtxStream::operator cudaStream_t() const {
+    for (const auto& b : g_bound)
+        if (b.first == id_) return b.second;
+    return last_.load();
+}
+void CtxStream::set(cudaStream_t s) {
+    g_bound.erase(std::remove_if(g_bound.begin(), g_bound.end(), [&](const auto& b) { return b.first == id_; }), g_bound.end());
+    last_.store(s);
+}
+void CtxStream::bind(cudaStream_t s) {
+    last_.store(s);
+    for (auto& b : g_bound)
+        if (b.first == id_) {
+            b.second = s;
+            return;
+        }
+    g_bound.emplace_back(id_, s);
+}
+uint64_t CtxStream::next_id() {
+    static std::atomic<uint64_t> n{0};
+    return n++;
+}
 
 // ---------------------------------------------------------------------------
 // Codecs
@@ -343,7 +370,7 @@ int at_ctx_create(int device, at_ctx** out) {
         // A blocking stream: it orders itself after work on the legacy default
         // stream (where host frameworks enqueue by default) and vice versa.
         AT_CUDA(cudaStreamCreateWithFlags(&c->own_stream, cudaStreamDefault));
-        c->stream = c->own_stream;
+        c->stream.set(c->own_stream);
         AT_CUDA(cudaDeviceGetAttribute(&c->num_sms, cudaDevAttrMultiProcessorCount, device));
         *out = c;
     });
@@ -366,7 +393,14 @@ int at_ctx_stream(at_ctx* ctx, void** stream) {
 int at_ctx_set_stream(at_ctx* ctx, void* stream) {
     return guard([&] {
         AT_REQUIRE(ctx, AT_ERR_INVALID_ARG, "null context");
-        ctx->stream = stream ? static_cast<cudaStream_t>(stream) : ctx->own_stream;
+        ctx->stream.set(stream ? static_cast<cudaStream_t>(stream) : ctx->own_stream);
+    });
+}
+
+int at_ctx_bind_stream(at_ctx* ctx, void* stream) {
+    return guard([&] {
+        AT_REQUIRE(ctx, AT_ERR_INVALID_ARG, "null context");
+        ctx->stream.bind(stream ? static_cast<cudaStream_t>(stream) : ctx->own_stream);
     });
 }
 

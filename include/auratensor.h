@@ -80,6 +80,10 @@ int at_ctx_stream(at_ctx* ctx, void** stream);
 /* Makes the context launch on `stream` (a cudaStream_t of the same device, for
  * example the host framework's current stream); NULL restores its own stream. */
 int at_ctx_set_stream(at_ctx* ctx, void* stream);
+/* The same for the calling thread: its launches stay on `stream` whatever other
+ * threads bind, until it calls this or at_ctx_set_stream again. Threads that
+ * have bound nothing launch on the stream that either call gave last. */
+int at_ctx_bind_stream(at_ctx* ctx, void* stream);
 
 /* ---- memory: Tensor.allocate / wrap / close (core/Tensor.java:88-120,234-239) */
 int at_alloc(at_ctx* ctx, size_t bytes, void** dptr);

@@ -1,0 +1,100 @@
+"""Operators called from several threads and streams."""
+import ctypes as C
+import threading
+
+import pytest
+import torch
+
+from auratensor_b200 import _lib
+from auratensor_b200.core import context
+
+pytestmark = pytest.mark.gpu
+
+
+def stream_of(ctx):
+    s = C.c_void_p()
+    _lib.call("at_ctx_stream", ctx, C.byref(s))
+    return s.value
+
+
+def in_threads(*steps):
+    """Runs lists of callables, one list per thread, step by step in turn; raises what they raise."""
+    barrier, errors = threading.Barrier(len(steps), timeout=60), []
+
+    def work(i):
+        try:
+            for j in range(max(map(len, steps))):
+                for who in range(len(steps)):
+                    barrier.wait()
+                    if who == i and j < len(steps[i]):
+                        steps[i][j]()
+        except BaseException as e:  # noqa: BLE001
+            errors.append(e)
+            barrier.abort()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(steps))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for e in errors:
+        if not isinstance(e, threading.BrokenBarrierError):
+            raise e
+
+
+def test_a_context_is_bound_per_thread(cuda):
+    """Thread B's call does not move thread A's launches to B's stream."""
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    seen = {}
+
+    def bind(i):
+        with torch.cuda.stream(streams[i]):
+            context(0)
+
+    def look(i):
+        seen[i] = stream_of(context_of)
+
+    context_of = context(0)
+    in_threads(*[[lambda i=i: bind(i), lambda i=i: look(i)] for i in range(2)])
+    assert seen == {i: streams[i].cuda_stream for i in range(2)}
+
+
+def test_a_thread_that_never_bound_the_context_takes_the_last_binding(cuda):
+    s, seen = torch.cuda.Stream(), []
+    with torch.cuda.stream(s):
+        ctx = context(0)
+    t = threading.Thread(target=lambda: seen.append(stream_of(ctx)))
+    t.start()
+    t.join()
+    assert seen == [s.cuda_stream]
+    context(0)
+
+
+def test_a_direct_binding_does_not_outlast_the_next_call(cuda):
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(a):
+        ctx = context(0)
+        _lib.call("at_ctx_set_stream", ctx, b.cuda_stream)
+        assert stream_of(ctx) == b.cuda_stream
+        context(0)
+        assert stream_of(ctx) == a.cuda_stream
+    context(0)
+
+
+def test_clashing_bindings_heal(cuda):
+    """Many rebindings at once: afterwards each thread still launches on its own stream."""
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(3000):
+                if stream_of(context(0)) != streams[i].cuda_stream:
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
