@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import threading
 
 import torch
 
@@ -139,7 +140,7 @@ class BlockKvCache:
         self._c = [KvBlocksC(code, self.headCountKv, self.headDim, self.blockTokens, self.nBlocks, self.maxSeqs, self.maxBlocks, 0,
                              *(at if l == 0 else [p + l * s for p, s in zip(at, step)]), *none, *shared) for l in range(self.layers)]
         self._refs = [C.addressof(c) for c in self._c]
-        self._ws: dict = {}  # attention workspaces by stream
+        self._ws = threading.local()  # attention workspaces by thread and stream
         self._scale = 1.0 / math.sqrt(self.headDim)
         self._free = None
         self._pages = None
@@ -232,13 +233,15 @@ class BlockKvCache:
                 _bad(f"expected a tensor on {self.device}, got {t.device}")
 
     def _workspace(self, stream: int, need: int) -> torch.Tensor:
-        """At least `need` bytes that calls on this stream share (they run one
-        after the other). A captured graph gets memory of its own."""
+        """At least `need` bytes that this thread's calls on this stream share
+        (they run one after the other; another thread's launches may come
+        between a call's two kernels). A captured graph gets memory of its own."""
         if torch.cuda.is_current_stream_capturing():
             return torch.empty(need, dtype=torch.uint8, device=self.device)
-        ws = self._ws.get(stream)
+        mine = self._ws.__dict__
+        ws = mine.get(stream)
         if ws is None or ws.numel() < need:
-            ws = self._ws[stream] = torch.empty(need, dtype=torch.uint8, device=self.device)
+            ws = mine[stream] = torch.empty(need, dtype=torch.uint8, device=self.device)
         return ws
 
     def append(self, layer: int, batch: TokenBatch, k: torch.Tensor, v: torch.Tensor) -> None:

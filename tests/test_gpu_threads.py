@@ -7,6 +7,7 @@ import torch
 
 from auratensor_b200 import _lib
 from auratensor_b200.core import context
+from auratensor_b200.kvblock import BlockKvCache, TokenBatch
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +99,50 @@ def test_clashing_bindings_heal(cuda):
     for t in threads:
         t.join()
     assert not wrong
+
+
+def split_batch(cuda, seed):
+    """A cache whose one long sequence is split over blocks that a second kernel joins (a workspace), and its query."""
+    cache = BlockKvCache.allocate(1, 150, 1, 64, 1, 150, 64, torch.float32)
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    k, v = (torch.randn((9001, 1, 64), generator=g, device=cuda) for _ in range(2))
+    cache.reserve(0, 9001)
+    cache.append(0, TokenBatch.of([0], [0], [9001]), k, v)
+    batch = TokenBatch.of([0], [9000], [1])
+    need = C.c_size_t()
+    _lib.call("at_kvb_attention_workspace", context(0), cache._refs[0], batch._ref, 4, 0, C.byref(need))
+    assert need.value > 0
+    return cache, batch, [torch.randn((1, 4, 64), generator=g, device=cuda) for _ in range(4)]
+
+
+def test_threads_on_one_stream_do_not_share_a_workspace(cuda):
+    """A call launches two kernels; another thread's may come between them."""
+    cache, batch, qs = split_batch(cuda, 1)
+    at = {}
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def note(i):
+        at[i] = cache._workspace(stream, 1 << 16).data_ptr()
+
+    in_threads([lambda: note(0), lambda: note(0)], [lambda: note(1), lambda: note(1)])
+    assert at[0] != at[1]
+
+
+def test_attention_from_several_threads(cuda):
+    cache, batch, qs = split_batch(cuda, 2)
+    want = [cache.attention(0, batch, q) for q in qs]
+    torch.cuda.synchronize()
+    got = [[] for _ in qs]
+
+    def work(i):
+        for _ in range(300):
+            got[i].append(cache.attention(0, batch, qs[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(qs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for w, ys in zip(want, got):
+        assert len(ys) == 300 and all(torch.equal(w, y) for y in ys)
