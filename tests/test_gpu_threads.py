@@ -146,3 +146,40 @@ def test_attention_from_several_threads(cuda):
     torch.cuda.synchronize()
     for w, ys in zip(want, got):
         assert len(ys) == 300 and all(torch.equal(w, y) for y in ys)
+
+
+def test_split_attention_on_several_streams(cuda):
+    """Different data on each stream: a workspace that two streams shared would mix them."""
+    cache, batch, qs = split_batch(cuda, 3)
+    want = [cache.attention(0, batch, q) for q in qs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in qs], []
+    for _ in range(50):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i, cache.attention(0, batch, qs[i])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(want[i], y) for i, y in got)
+
+
+def test_captured_split_attention_keeps_its_workspace(cuda):
+    """Calls outside the graph, and memory freed and taken again after the capture, do not touch the graph's workspace."""
+    cache, batch, qs = split_batch(cuda, 4)
+    want = [cache.attention(0, batch, q) for q in qs]
+    q = qs[0].clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = cache.attention(0, batch, q)
+    side = torch.cuda.Stream()
+    for i in range(40):
+        j = i % 4
+        q.copy_(qs[j])
+        side.wait_stream(torch.cuda.current_stream())
+        graph.replay()
+        with torch.cuda.stream(side):
+            other = cache.attention(0, batch, qs[(j + 1) % 4])
+            del_me = torch.full((1 << 20,), float("nan"), device=cuda)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[j]) and torch.equal(other, want[(j + 1) % 4])
+        del del_me
