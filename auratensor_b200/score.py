@@ -21,6 +21,7 @@ import numpy as np
 import torch
 
 from . import synth
+from ._lib import AT_ERR_INVALID_ARG, AT_ERR_STATE, IllegalArgumentException, IllegalStateException
 from .core import DType, Kernels, Tensor
 from .gguf import GgufFile
 from .inference import LlamaConfig, LlamaModel
@@ -84,10 +85,22 @@ class BlockLlama:
         a, b = x[..., 0::2], x[..., 1::2]
         return torch.stack((a * cos - b * sin, b * cos + a * sin), dim=-1).flatten(-2)
 
+    def _check(self, sequences) -> None:
+        """What LlamaModel refuses: ids and positions index tables on the device."""
+        for _, start, toks in sequences:
+            bad = next((t for t in toks if not 0 <= int(t) < self.config.vocabSize), None)
+            if bad is not None:
+                raise IllegalArgumentException(AT_ERR_INVALID_ARG, f"token id {bad} out of range")
+            if start < 0:
+                raise IllegalArgumentException(AT_ERR_INVALID_ARG, "negative position")
+            if start + len(toks) > self.config.contextLength:
+                raise IllegalStateException(AT_ERR_STATE, f"position {start + len(toks) - 1} exceeds maxContext {self.config.contextLength}")
+
     def forward(self, sequences) -> torch.Tensor:
         """sequences: [(slot, start, token ids)], one run of consecutive tokens
         each; reserves their pages, appends them and returns the logits of every
         token, [tokens][vocab] on the device."""
+        self._check(sequences)
         c, hd = self.config, self.config.headDim()
         slots, starts = [s for s, _, _ in sequences], [p for _, p, _ in sequences]
         counts = [len(t) for _, _, t in sequences]
