@@ -52,6 +52,7 @@
 // though they save a TMEM load: 347 us.
 // Every wait is bounded: one that runs out sets the status bit, and all roles
 // leave.
+#include <atomic>
 #include <cstdint>
 #include <string>
 #include <type_traits>
@@ -754,13 +755,17 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
 template <class T, int HD>
 void prompt_launch(PromptParams p, cudaStream_t s) {
     auto kern = kvb_attn_prompt_kernel<T, HD>;
-    static const int regs = [&] {  // per instance
+    static std::atomic<uint64_t> ready{0};  // per instance: the devices it was set up on (the attribute is a device's)
+    int dev = 0;
+    AT_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
+    if (!(ready.load() & bit)) {
         AT_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pr_smem<T, HD>()));
         cudaFuncAttributes a;
         AT_CUDA(cudaFuncGetAttributes(&a, kern));
-        return a.numRegs;
-    }();
-    AT_REQUIRE(regs == pr_launch_regs<T>(), AT_ERR_CUDA, "prompt attention was built with another register count than its warpgroups share");
+        AT_REQUIRE(a.numRegs == pr_launch_regs<T>(), AT_ERR_CUDA, "prompt attention was built with another register count than its warpgroups share");
+        ready.fetch_or(bit);
+    }
     const int per = pr_tiles<T>() * (PR_ROWS / p.G);
     p.blocks = (int)(((int64_t)p.b.max_tokens + per - 1) / per);
     const int64_t grid = (int64_t)p.blocks * p.c.hkv * p.b.n_seqs;
