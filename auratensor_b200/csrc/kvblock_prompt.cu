@@ -107,6 +107,20 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, PrShare
     *reinterpret_cast<volatile int*>(&sh->bad) = 1;
     return false;
 }
+// The same, not cut short by another role's failure: for what must be over
+// before the block may leave.
+__device__ __forceinline__ void bar_drain(uint64_t* bar, uint32_t parity, PrShared* sh) {
+    for (int it = 0; it < kPrSpinLimit; ++it) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (ok) return;
+    }
+    *reinterpret_cast<volatile int*>(&sh->bad) = 1;
+}
 
 template <int N>
 __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -741,7 +755,7 @@ __global__ void __launch_bounds__(pr_threads<T>(), 1) kvb_attn_prompt_kernel(con
             for (int k = lo; k <= hi && ok; ++k) ok = (k - lo) & 1 ? step(k, c1, c0) : step(k, c0, c1);
         }
         mma_commit(&sh.o_done, leader);
-        wait(&sh.o_done, 0);  // nothing in flight when TMEM is freed
+        bar_drain(&sh.o_done, 0, &sh);  // nothing in flight when TMEM is freed, also after a wait that ran out
         }
     }
     }  // placed
