@@ -148,6 +148,7 @@ SIGNATURES = {
     "at_model_forward_prompt": [_vp, _vp, _i],
     "at_model_forward_batch": [_vp, _vp, _vp, _i, _vp],
     "at_model_logits_device": [_vp, _PP],
+    "at_model_logits_rows": [_vp, C.POINTER(C.c_int)],
     "at_model_argmax": [_vp, _i, _vp],
     "at_model_step_kernel": [_vp, _vp],
     "at_model_step_stamps": [_vp, _i, _i64, _vp, _i64, _vp],

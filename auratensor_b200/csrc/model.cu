@@ -1168,6 +1168,7 @@ struct at_model {
     unsigned long long* d_argkey = nullptr;  // packed (value, index) max per row
     int* h_tokens = nullptr;      // pinned
     int64_t* h_pos = nullptr;     // pinned
+    int logits_rows = 0;          // rows of `logits` that the last step computed
     int nchunk_max = 0;
     int64_t slot_stride = 0;      // floats per KV slot (all layers)
     std::vector<int64_t> kv_size;
@@ -1651,6 +1652,7 @@ void run_step_enqueue_only(at_model* m, const int* tokens, const int64_t* positi
         if (!m->graph[B]) m->graph[B] = capture(m, enqueue_step, B);
         AT_CUDA(cudaGraphLaunch(m->graph[B], c->stream));
     }
+    m->logits_rows = B;
 }
 
 void run_step(at_model* m, const int* tokens, const int64_t* positions, int B, float* logits_host) {
@@ -2578,6 +2580,7 @@ int at_model_generate(at_model* m, int first_token, int64_t start_pos, int n_ste
             if (!m->graph_gen) m->graph_gen = capture(m, enqueue_generate_step, 1);
             for (int i = 0; i < n_steps; ++i) AT_CUDA(cudaGraphLaunch(m->graph_gen, c->stream));
         }
+        m->logits_rows = 1;
         m->kv_size[0] = std::max<int64_t>(m->kv_size[0], start_pos + n_steps);
         if (c->world > 1)
             AT_CUDA(cudaMemcpyAsync(m->h_ar_err, m->d_ar_err, sizeof(int), cudaMemcpyDeviceToHost, c->stream));
@@ -2750,6 +2753,7 @@ int at_model_generate_sampled(at_model* m, int batch, const int* first_tokens, c
         AT_CUDA(cudaMemsetAsync(m->d_step_ctr, 0, sizeof(int), c->stream));
         if (!m->graph_samp[batch]) m->graph_samp[batch] = capture(m, enqueue_sampled_step, batch);
         for (int i = 0; i < n_steps; ++i) AT_CUDA(cudaGraphLaunch(m->graph_samp[batch], c->stream));
+        m->logits_rows = batch;
         if (c->world > 1)
             AT_CUDA(cudaMemcpyAsync(m->h_ar_err, m->d_ar_err, sizeof(int), cudaMemcpyDeviceToHost, c->stream));
         if (tokens_out_host)
@@ -2865,6 +2869,7 @@ int at_model_profile_batch(at_model* m, int batch, const int* tokens, const int6
             m->graph_prof_batch = batch;
         }
         AT_CUDA(cudaGraphLaunch(m->graph_prof, c->stream));
+        m->logits_rows = batch;
         if (c->world > 1)
             AT_CUDA(cudaMemcpyAsync(m->h_ar_err, m->d_ar_err, sizeof(int), cudaMemcpyDeviceToHost, c->stream));
         AT_CUDA(cudaStreamSynchronize(c->stream));
@@ -2888,6 +2893,13 @@ int at_model_logits_device(at_model* m, float** logits_dev) {
     return guard([&] {
         AT_REQUIRE(m && logits_dev && m->finalized, AT_ERR_INVALID_ARG, "bad argument");
         *logits_dev = m->logits;
+    });
+}
+
+int at_model_logits_rows(const at_model* m, int* rows) {
+    return guard([&] {
+        AT_REQUIRE(m && rows && m->finalized, AT_ERR_INVALID_ARG, "bad argument");
+        *rows = m->logits_rows;
     });
 }
 
@@ -2926,6 +2938,7 @@ int at_model_step_stamps(at_model* m, int token, int64_t position, unsigned long
         AT_CUDA(cudaMemcpyAsync(m->d_tokens, m->h_tokens, sizeof(int), cudaMemcpyHostToDevice, c->stream));
         AT_CUDA(cudaMemcpyAsync(m->d_pos, m->h_pos, sizeof(int64_t), cudaMemcpyHostToDevice, c->stream));
         ds_launch(m, false);
+        m->logits_rows = 1;
         AT_CUDA(cudaMemcpyAsync(m->h_ds_err, m->ds_err, sizeof(int), cudaMemcpyDeviceToHost, c->stream));
         AT_CUDA(cudaMemcpyAsync(stamps_host, m->ds_stamps, (size_t)need * sizeof(unsigned long long),
                                 cudaMemcpyDeviceToHost, c->stream));

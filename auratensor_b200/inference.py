@@ -217,11 +217,19 @@ class LlamaModel:
     def logProbs(self, tokenIds=None, top: int = 0) -> "LogProbs":
         """Log probabilities on the device of the last step's logits rows
         0..len(tokenIds)-1 (row 0 without tokens): of the given tokens, with
-        the entropy and `top` alternatives (scoring.LogProbs)."""
+        the entropy and `top` alternatives (scoring.LogProbs). Rows that the
+        last step did not compute are refused; a prompt is no step, it leaves
+        the logits alone. Sampling with a repetition penalty changes them in
+        place, as the reference's Sampler does: after such a step the scores are
+        those of the penalised logits."""
         from .scoring import LogProbs
         rows = 1 if tokenIds is None else len(tokenIds)
         if not 1 <= rows <= self.max_batch:
             raise _lib.IllegalArgumentException(_lib.AT_ERR_INVALID_ARG, f"1 to {self.max_batch} rows, got {rows}")
+        have = C.c_int()
+        call("at_model_logits_rows", self._h, C.byref(have))
+        if rows > have.value:
+            raise _lib.IllegalStateException(_lib.AT_ERR_STATE, f"the last step computed {have.value} rows of logits, {rows} are asked for")
         logits = self.logitsDevice()[:rows]
         ids = None if tokenIds is None else torch.as_tensor(tokenIds, dtype=torch.int32).to(logits.device)
         return LogProbs.of(logits, ids, top)

@@ -232,6 +232,9 @@ int at_model_forward_batch(at_model* m, const int* tokens, const int64_t* positi
                            float* logits_host);
 /* Device address of the last step's logits [max_batch][vocab] (full vocab on every rank). */
 int at_model_logits_device(at_model* m, float** logits_dev);
+/* How many of their rows the last step computed (0 before the first; the rows
+ * after them are an earlier step's). Batched prompts compute no logits. */
+int at_model_logits_rows(const at_model* m, int* rows);
 /* Greedy token of each of the last step's `batch` rows (Sampler greedy path,
  * inference/Sampler.java:56-67: first index of the maximum). */
 int at_model_argmax(at_model* m, int batch, int* tokens_host);
