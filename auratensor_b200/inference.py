@@ -125,6 +125,17 @@ class KVCache:
         call("at_model_kv_reset", self._m._h, self._slot)
 
 
+def _stream_of(ctx: int) -> int:
+    s = C.c_void_p()
+    call("at_ctx_stream", ctx, C.byref(s))
+    return s.value or 0
+
+
+def _after(stream: int, other: int, device: int) -> None:
+    """What is launched on `stream` from now on waits for what `other` has now."""
+    torch.cuda.ExternalStream(stream, device=device).wait_stream(torch.cuda.ExternalStream(other, device=device))
+
+
 class LlamaModel:
     """inference/LlamaModel.java:41-381 on the device.
 
@@ -133,6 +144,7 @@ class LlamaModel:
     may be numpy arrays / bytes (uploaded once) or uint8 CUDA tensors.
     Under tensor parallelism pass ``ctx`` from ``tp.init_tp_context``.
     """
+    _unfinished: int | None = None  # the stream of the last generate that was not waited for
 
     def __init__(self, config: LlamaConfig, tensors: dict | None = None, max_batch: int = 1, ctx=None,
                  world: int = 1, layout: int = 0, kv_type: int = 0):
@@ -232,12 +244,26 @@ class LlamaModel:
             raise _lib.IllegalStateException(_lib.AT_ERR_STATE, f"the last step computed {have.value} rows of logits, {rows} are asked for")
         logits = self.logitsDevice()[:rows]
         ids = None if tokenIds is None else torch.as_tensor(tokenIds, dtype=torch.int32).to(logits.device)
-        return LogProbs.of(logits, ids, top)
+        # The step may have run, or still run (generate without waiting), on a
+        # stream that is not the scores'; the next step overwrites the logits.
+        # A captured graph's scores are ordered by whoever replays it.
+        device = logits.device.index
+        steps = {_stream_of(self._ctx), self._unfinished}
+        here = _stream_of(context(device))
+        if torch.cuda.is_current_stream_capturing():
+            return LogProbs.of(logits, ids, top)
+        for s in steps - {here, None}:
+            _after(here, s, device)
+        r = LogProbs.of(logits, ids, top)
+        if _stream_of(self._ctx) != here:
+            _after(_stream_of(self._ctx), here, device)
+        return r
 
     def generate(self, firstToken: int, startPos: int, nSteps: int, wait: bool = True) -> np.ndarray | None:
         """Greedy decode of slot 0 on the device: nSteps tokens, no host round trip per step."""
         if not wait:
             call("at_model_generate", self._h, int(firstToken), int(startPos), int(nSteps), None)
+            self._unfinished = _stream_of(self._ctx)
             return None
         out = np.empty(max(1, nSteps), dtype=np.int32)
         call("at_model_generate", self._h, int(firstToken), int(startPos), int(nSteps),
