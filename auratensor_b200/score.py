@@ -30,7 +30,7 @@ from .quant import ORIENT_N, ORIENT_T, Q4_0, Q8_0, QMatrix
 from .scoring import LogProbs
 
 _CODECS = {Q4_0.TYPE: Q4_0, Q8_0.TYPE: Q8_0}
-GEMV_ROWS = 8  # up to so many tokens at once the projections run in FP32 (GEMV), above on the tensor cores (bf16)
+GEMV_ROWS = 8  # tokens that one FP32 projection (GEMV) takes at a time
 
 
 def _f32(t: dict, device) -> torch.Tensor:
@@ -40,9 +40,17 @@ def _f32(t: dict, device) -> torch.Tensor:
 
 class BlockLlama:
     """A Llama-family model over a BlockKvCache. tensors: {name: {"type", "data"}}
-    in the reference's layout (Q4_0 or Q8_0 matrices, F32 norms)."""
+    in the reference's layout (Q4_0 or Q8_0 matrices, F32 norms). projections:
+    "auto" multiplies in FP32 while a call has at most 8 tokens and on the
+    tensor cores (bf16 operands) above, so a token's logits move in the third
+    digit with how many others share the call; "f32" always multiplies in FP32,
+    8 tokens at a time, as LlamaModel's steps do."""
 
-    def __init__(self, config: LlamaConfig, tensors: dict, nBlocks: int, maxSeqs: int, blockTokens: int = 64, device=None):
+    def __init__(self, config: LlamaConfig, tensors: dict, nBlocks: int, maxSeqs: int, blockTokens: int = 64, device=None,
+                 projections: str = "auto"):
+        if projections not in ("auto", "f32"):
+            raise IllegalArgumentException(AT_ERR_INVALID_ARG, f"projections must be auto or f32, got {projections}")
+        self.projections = projections
         self.config = c = config
         self.device = dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         hd, d = c.headDim(), c.embeddingLength
@@ -74,8 +82,17 @@ class BlockLlama:
         per_seq = -(-c.contextLength // blockTokens)
         self.cache = BlockKvCache.allocate(c.blockCount, nBlocks, c.headCountKv, hd, maxSeqs, per_seq, blockTokens, torch.float32, dev)
 
-    def _project(self, m: QMatrix, x: torch.Tensor) -> torch.Tensor:
-        return m.gemv(x) if x.shape[0] <= GEMV_ROWS else m.gemm(x)
+    def _project(self, m: QMatrix, x: torch.Tensor, tokens: int | None = None) -> torch.Tensor:
+        """x: all of a call's tokens, or some of `tokens`."""
+        n = x.shape[0]
+        if self.projections == "auto" and (tokens or n) > GEMV_ROWS:
+            return m.gemm(x)
+        if n <= GEMV_ROWS:
+            return m.gemv(x)
+        y = torch.empty((n, m.out_features), dtype=torch.float32, device=x.device)
+        for i in range(0, n, GEMV_ROWS):
+            m.gemv(x[i:i + GEMV_ROWS], y[i:i + GEMV_ROWS])
+        return y
 
     def _norm(self, x: torch.Tensor, w: torch.Tensor) -> None:
         Kernels.rmsNormInPlace(Tensor.wrap(x, DType.FP32, x.shape), Tensor.wrap(w, DType.FP32, w.shape), self.config.rmsNormEpsilon)
@@ -100,6 +117,11 @@ class BlockLlama:
         """sequences: [(slot, start, token ids)], one run of consecutive tokens
         each; reserves their pages, appends them and returns the logits of every
         token, [tokens][vocab] on the device."""
+        x = self._hidden(sequences)
+        return self._project(self.head, x)
+
+    def _hidden(self, sequences) -> torch.Tensor:
+        """forward up to the output matrix."""
         self._check(sequences)
         c, hd = self.config, self.config.headDim()
         slots, starts = [s for s, _, _ in sequences], [p for _, p, _ in sequences]
@@ -125,22 +147,23 @@ class BlockLlama:
             Kernels.siluInPlaceSegment(g, g.numel())
             x = x + self._project(w["down"], g * self._project(w["up"], x))
         self._norm(x, self.out_norm)
-        return self._project(self.head, x)
+        return x
 
     def score(self, texts, top: int = 0, chunk: int = 512):
         """Log probabilities of each text's tokens 1.. given those before them
-        (LogProbs per text), in slots 0.., `chunk` tokens of each per call."""
+        (LogProbs per text), in slots 0.., `chunk` tokens of each per call. The
+        logits of one text's chunk are held at a time."""
         for slot in range(len(texts)):
             self.cache.release(slot)
         parts = [[] for _ in texts]
         longest = max(len(t) for t in texts)
         for at in range(0, longest, chunk):
             runs = [(s, at, t[at:at + chunk]) for s, t in enumerate(texts) if len(t) > at]
-            logits, row = self.forward(runs), 0
+            x, row = self._hidden(runs), 0
             for slot, start, toks in runs:
                 follow = torch.tensor([int(t) for t in texts[slot][start + 1:start + len(toks) + 1]], dtype=torch.int32).to(self.device)
                 if follow.numel():
-                    parts[slot].append(LogProbs.of(logits[row:row + follow.numel()], follow, top))
+                    parts[slot].append(LogProbs.of(self._project(self.head, x[row:row + follow.numel()], x.shape[0]), follow, top))
                 row += len(toks)
 
         def cat(xs):
@@ -158,6 +181,8 @@ def main(argv=None) -> None:
     ap.add_argument("--tokens", type=int, default=60, help="length of the longest random text")
     ap.add_argument("--texts", type=int, default=4)
     ap.add_argument("--block", type=int, default=64, help="tokens per cache block: 16, 32, 64 or 128")
+    ap.add_argument("--projections", default="f32", choices=["f32", "bf16"],
+                    help="f32: as the FP32 cache's model, so that the difference is the cache's; bf16: prompts on the tensor cores")
     args = ap.parse_args(argv)
     torch.cuda.set_device(0)
     if args.gguf:
@@ -178,7 +203,7 @@ def main(argv=None) -> None:
     texts = ([[int(t) for t in args.ids.split(",")]] if args.ids else
              [rng.integers(0, cfg.vocabSize, size=max(2, args.tokens - 7 * i)).tolist() for i in range(args.texts)])
     blocks = sum(-(-len(t) // args.block) for t in texts)
-    model = BlockLlama(cfg, tensors, blocks, len(texts), args.block)
+    model = BlockLlama(cfg, tensors, blocks, len(texts), args.block, projections="f32" if args.projections == "f32" else "auto")
     scores = model.score(texts)
     model.cache.check()
     # the same texts through the FP32 cache, token by token
@@ -194,7 +219,7 @@ def main(argv=None) -> None:
     got = torch.cat([s.logProb for s in scores])
     per_token = 2 * cfg.blockCount * cfg.headCountKv * (cfg.headDim() + 4 / args.block)
     print(json.dumps({
-        "model": args.gguf or args.model, "texts": [len(t) for t in texts], "block_tokens": args.block,
+        "model": args.gguf or args.model, "texts": [len(t) for t in texts], "block_tokens": args.block, "projections": args.projections,
         "mean_log_prob": round(float(got.mean()), 6), "mean_log_prob_f32_cache": round(float(torch.cat(exact).mean()), 6),
         "max_difference": round(float((got - torch.cat(exact)).abs().max()), 6),
         "mean_entropy": round(float(torch.cat([s.entropy for s in scores]).mean()), 6),
