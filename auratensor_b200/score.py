@@ -151,12 +151,13 @@ class BlockLlama:
 
     def score(self, texts, top: int = 0, chunk: int = 512):
         """Log probabilities of each text's tokens 1.. given those before them
-        (LogProbs per text), in slots 0.., `chunk` tokens of each per call. The
-        logits of one text's chunk are held at a time."""
+        (LogProbs per text, None for a text of less than two), in slots 0..,
+        `chunk` tokens of each per call. The logits of one text's chunk are held
+        at a time."""
         for slot in range(len(texts)):
             self.cache.release(slot)
         parts = [[] for _ in texts]
-        longest = max(len(t) for t in texts)
+        longest = max((len(t) for t in texts), default=0)
         for at in range(0, longest, chunk):
             runs = [(s, at, t[at:at + chunk]) for s, t in enumerate(texts) if len(t) > at]
             x, row = self._hidden(runs), 0
@@ -184,6 +185,10 @@ def main(argv=None) -> None:
     ap.add_argument("--projections", default="f32", choices=["f32", "bf16"],
                     help="f32: as the FP32 cache's model, so that the difference is the cache's; bf16: prompts on the tensor cores")
     args = ap.parse_args(argv)
+    if args.texts < 1:
+        ap.error("--texts must be at least 1")
+    if args.ids is not None and len(args.ids.split(",")) < 2:
+        ap.error("--ids needs two ids at least: each but the first is scored")
     torch.cuda.set_device(0)
     if args.gguf:
         with GgufFile.open(args.gguf) as g:
@@ -200,7 +205,7 @@ def main(argv=None) -> None:
         gen = torch.Generator(device="cuda").manual_seed(0)
         tensors = {n: {"type": t, "data": synth.generate_torch_tensor(dims, t, gen, "cuda")} for n, dims, t in shape.tensor_dims()}
     rng = np.random.default_rng(1)
-    texts = ([[int(t) for t in args.ids.split(",")]] if args.ids else
+    texts = ([[int(t) for t in args.ids.split(",")]] if args.ids is not None else
              [rng.integers(0, cfg.vocabSize, size=max(2, args.tokens - 7 * i)).tolist() for i in range(args.texts)])
     blocks = sum(-(-len(t) // args.block) for t in texts)
     model = BlockLlama(cfg, tensors, blocks, len(texts), args.block, projections="f32" if args.projections == "f32" else "auto")

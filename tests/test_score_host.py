@@ -3,7 +3,7 @@ import pytest
 
 from auratensor_b200 import _lib
 from auratensor_b200.inference import LlamaConfig
-from auratensor_b200.score import BlockLlama
+from auratensor_b200.score import BlockLlama, main
 from auratensor_b200.synth import TINY
 
 
@@ -32,3 +32,14 @@ def test_positions_past_the_context_are_refused(start, n):
         model().forward([(0, start, [1] * n)])
     with pytest.raises(_lib.IllegalArgumentException, match="negative"):
         model().forward([(0, -1, [1])])
+
+
+@pytest.mark.parametrize("args", [["--ids", "5"], ["--ids", ""], ["--texts", "0"], ["--texts", "-1"]])
+def test_a_command_with_nothing_to_score_is_refused(args, capsys):
+    with pytest.raises(SystemExit) as e:
+        main(args)
+    assert e.value.code == 2 and "at least" in capsys.readouterr().err
+
+
+def test_no_texts_have_no_scores():
+    assert model().score([]) == []
