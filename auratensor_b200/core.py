@@ -16,7 +16,7 @@ import threading
 import torch
 
 from . import _lib
-from ._lib import IllegalArgumentException, call
+from ._lib import IllegalArgumentException, call, lib
 
 
 class DType(enum.Enum):
@@ -57,7 +57,7 @@ def context(device: int | None = None) -> int:
                 p = C.c_void_p()
                 call("at_ctx_create", device, C.byref(p))
                 ctx = _ctxs[device] = p.value
-    rc = _lib.lib().at_ctx_bind_stream(ctx, _current_stream(device))
+    rc = lib().at_ctx_bind_stream(ctx, _current_stream(device))
     if rc:
         _lib.check(rc)
     return ctx

@@ -64,9 +64,8 @@ class TokenBatch:
             _bad("batch tensors must be on one device")
         if not (slots.is_contiguous() and starts.is_contiguous() and offsets.is_contiguous()):
             _bad("batch tensors must be contiguous")
-        for name, x, most in (("nTokens", nTokens, INT32_MAX), ("maxTokens", maxTokens, INT32_MAX), ("maxEnd", maxEnd, INT64_MAX)):
-            if not 0 <= x <= most:
-                _bad(f"{name} must be in [0, {most}], got {x}")
+        if not (0 <= nTokens <= INT32_MAX and 0 <= maxTokens <= INT32_MAX and 0 <= maxEnd <= INT64_MAX):
+            _bad(f"nTokens and maxTokens must be in [0, {INT32_MAX}], maxEnd in [0, {INT64_MAX}], got {nTokens}, {maxTokens}, {maxEnd}")
         self.slots, self.starts, self.offsets = slots, starts, offsets
         self.nSeqs, self.nTokens, self.maxTokens, self.maxEnd = n, int(nTokens), int(maxTokens), int(maxEnd)
         self._c = TokenBatchC(n, self.nTokens, self.maxTokens, 0, self.maxEnd, slots.data_ptr(), starts.data_ptr(), offsets.data_ptr())
