@@ -128,6 +128,8 @@ class BlockKvCache:
                 _bad(f"{name} must be {dt} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
             if t.get_device() != index or not t.is_contiguous():
                 _bad(f"{name} must be contiguous and on the device of kBlocks")
+        if status is not None and (status.dtype != torch.int32 or status.numel() != 1 or status.get_device() != index):
+            _bad("status must be one int32 on the device of kBlocks")
         self.kBlocks, self.vBlocks, self.kScales, self.vScales, self.table = kBlocks, vBlocks, kScales, vScales, table
         self.kTail, self.vTail, self.kTailMax, self.vTailMax, self.status = kTail, vTail, kTailMax, vTailMax, status
         # layer l's buffers start l slices into each tensor

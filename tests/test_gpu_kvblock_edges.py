@@ -6,7 +6,7 @@ import torch
 
 import kvblock_ref as ref
 from auratensor_b200 import _lib
-from auratensor_b200.kvblock import TokenBatch
+from auratensor_b200.kvblock import BlockKvCache, TokenBatch
 from test_gpu_kvblock import BF16, F16, F32, ROUND, check_values, f32, f64, heads, new_cache
 
 pytestmark = pytest.mark.gpu
@@ -170,3 +170,17 @@ def test_sizes_that_do_not_fit_are_refused(cuda):
     for sizes in (((1 << 32) + 3, 3, 3), (3, (1 << 32) + 3, 3), (-1, 3, 3), (3, -1, 3), (3, 3, 1 << 64), (3, 3, -1)):
         with pytest.raises(_lib.IllegalArgumentException, match="must be in"):
             loose(b, *sizes)
+
+
+def test_a_status_word_that_the_kernels_cannot_write_is_refused(cuda):
+    """No call is made with these: a kernel would write to a host address."""
+    c = new_cache(F32, hd=64, block=32)
+    for status in (torch.zeros(1, dtype=torch.int32), torch.zeros(1, device=cuda), torch.zeros(0, dtype=torch.int32, device=cuda),
+                   torch.zeros(1, dtype=torch.int64, device=cuda)):
+        with pytest.raises(_lib.IllegalArgumentException, match="status"):
+            BlockKvCache.wrap(c.kBlocks, c.vBlocks, c.kScales, c.vScales, c.table, dtype=F32, status=status)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    w = BlockKvCache.wrap(c.kBlocks, c.vBlocks, c.kScales, c.vScales, c.table, dtype=F32, status=status)
+    w.read(0, TokenBatch.of([0], [0], [3]))  # nothing is reserved
+    with pytest.raises(_lib.IllegalStateException, match="outside the pool"):
+        w.check()
