@@ -157,7 +157,7 @@ struct AppendSrc {
 // read back: 120 us, 5.2 TB/s over both kernels; the write is bound by its
 // instructions (packed maxima, products and roundings fill 86 % of the issue
 // slots), not by memory. K and V of a block in one CTA spill: 125 us. One token
-// of one sequence, written and read back: 4.9 us, 0.4 of it the look at the
+// of one sequence, written and read back: 5.1 us, 0.4 of it the look at the
 // tail (held in eight values per lane that look took 57 registers for 48, a
 // CTA per SM, and 5 us of the prompts; a row spread over the warp takes none).
 template <class T, int HD, int NT, int NCH>
@@ -286,7 +286,7 @@ constexpr int READ_TOKENS = 64;  // positions per CTA
 // A CTA reads READ_TOKENS positions of one KV head, K or V, and writes them
 // token-major: 8 values per thread and row, all of its loads in flight at once.
 // Bound by memory traffic: 131071 tokens of 8 heads of 128 as F16: 135 us, 5.9
-// TB/s; 2048 tokens of 8 heads of 64 as FP32: 4.5 us.
+// TB/s; 2048 tokens of 8 heads of 64 as FP32: 5.4 us.
 template <class T, int HD>
 __global__ void __launch_bounds__(READ_THREADS) kvb_read_kernel(KvbDev c, KvbBatch b, T* __restrict__ ok, T* __restrict__ ov,
                                                                 int chunks) {

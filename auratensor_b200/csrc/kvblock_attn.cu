@@ -55,16 +55,19 @@ namespace cg = cooperative_groups;
 // 58 % of the integer pipe go to turning bytes into f16, with 12 warps per SM
 // to cover the loads. (K Q^T on the int8 form of mma.sync, with no work per key
 // byte: 142 us with queries as two int8 parts, which lose what is small beside
-// a row's largest value; 148 us with three, which do not.) One sequence of
-// 131072 tokens over 8 heads of 64: 39 us, 3.4 TB/s; of 513 tokens: 7.6 us, the
-// time of its launch and of three loads one after another.
+// a row's largest value; 148 us with three, which do not.) In FP32, with twice
+// the products and registers spilled (below): 229 us. One sequence of 131072
+// tokens over 8 heads of 64: 39 us, 3.4 TB/s; of 513 tokens: 7.6 us, the time
+// of its launch and of three loads one after another.
 constexpr int ST_WARPS = 4;
 constexpr int ST_THREADS = 32 * ST_WARPS;
 constexpr float ST_ROOM = 12.f;
 // Keys of a warp's unit: 8 KB of K and V each at a time. At head_dim 128 a
 // unit of 64 keys needs 252 registers and leaves two warps per scheduler to
-// cover each other's latencies (64 sequences up to 8191 tokens: 163 us); 32
-// keys fit 168 registers and three (149 us).
+// cover each other's latencies (64 sequences up to 8191 tokens: 163 us); with
+// 16-bit queries 32 keys fit 168 registers and three (149 us). FP32 queries do
+// not fit either: 180 bytes are spilled and 108 loaded again per thread with 8
+// rows, 256 and 212 of 255 registers with 16 (229 us).
 constexpr int st_unit(int hd) { return hd == 128 ? 32 : 64; }
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -630,6 +633,17 @@ void launch_step(const StepParams& p, const StepPlan& s, cudaStream_t st) {
     }
 }
 
+// Rows per KV head up to which the step kernel serves a sequence. It reads and
+// converts K and V once per 16 rows, the prompt kernel once per 256 (128 in
+// FP32), but only the step kernel splits the keys. 64 BF16 heads over 8 of 128,
+// us, step / prompt kernel (FP32 in brackets):
+//                              16 rows       32 rows       64 rows
+//    1 sequence, 512 tokens    9 / 19        10 / 19       11 / 19
+//    1 sequence, 32768        32 / 585       45 / 585      73 / 585   (108 / 639)
+//   16 sequences to 4096      41 / 83        71 / 83      129 / 84    (193 / 93)
+//   64 sequences to 4096     135 / 261      227 / 250     415 / 268   (648 / 298)
+// Up to 64 rows it is at most 2.2 times slower where many sequences fill the
+// GPU, and 8 times faster where one has to.
 constexpr int STEP_MAX_ROWS = 64;
 
 // The step kernel serves every sequence of at most STEP_MAX_ROWS query rows

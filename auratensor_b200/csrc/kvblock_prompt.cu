@@ -38,11 +38,13 @@
 // unpack); Q is stored alike and the output is put back in order.
 //
 // Two prompts up to 4096 tokens, 32 BF16 heads over 8 of 128: 321 us, 725
-// TFLOP/s of causal products, 45 % of a plain matrix product's rate; 512
-// tokens in FP32 (two products for one): 19 us. What bounds it: a tile of
-// 128 x 128 weights costs 1024 cycles of ex2 and 1024 of tensor work, and a
-// query tile's softmax, P V and next S follow one another (4500 cycles for two
-// tiles); 15 % of a block's time is its first loads and its last stores.
+// TFLOP/s of causal products, 45 % of a plain matrix product's rate; in FP32,
+// with two products for one, one query tile and a few spilled registers (28
+// bytes stored, 36 loaded at head_dim 128): 614 us, 512 tokens 21 us. What
+// bounds it: a tile of 128 x 128 weights costs 1024 cycles of ex2 and 1024 of
+// tensor work, and a query tile's softmax, P V and next S follow one another
+// (4500 cycles for two tiles); 15 % of a block's time is its first loads and
+// its last stores.
 // S in two buffers of 64 keys breaks that chain but pays for each product as
 // for one of 128 (415 us); releasing P in halves holds up the other tile's
 // products (332 us).

@@ -22,11 +22,14 @@
 // then they are left out and the first ids equal to tau fill up at the end. A
 // row is one CTA, or a cluster of up to 8 whose parts meet in distributed
 // shared memory when there are too few rows to fill the GPU.
-// 2048 rows of 128256 logits, k = 20: 138 us in BF16 (3.8 TB/s; the sums and the
-// comparison with tau cost more than the loads), 183 us in FP32 (5.7 TB/s). 8
-// rows of FP32, k = 5: 8.4 us, its launch, the list's ranking and the cluster's
-// join. 256 threads are as fast for many rows and slower for few (10.5 us); the
-// next step's loads ahead of time need 64 registers and lose a CTA (167 us).
+// 2048 rows of 128256 logits, k = 20: 139 us in BF16 (3.8 TB/s: 70 % of the
+// issue slots and 45 % of ex2's rate; the rest is waiting, at the CTA's
+// barriers and for a step's loads, which are not in flight while the step
+// before is summed or a row's list is ranked), 183 to 199 us in FP32 (5.5
+// TB/s). 8 rows of FP32, k = 5: 8.8 us, its launch, the list's ranking and the
+// cluster's join. 256 threads are as fast for many rows and slower for few
+// (10.5 us); the next step's loads ahead of time need 64 registers and lose a
+// CTA (167 us).
 #include <cooperative_groups.h>
 
 #include <cstdint>

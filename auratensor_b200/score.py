@@ -6,6 +6,7 @@ through ``LlamaModel`` with its FP32 cache.
     python -m auratensor_b200.score                                   # small synthetic model, 4 texts
     python -m auratensor_b200.score --model llama-3.2-1b --tokens 500 --block 32
     python -m auratensor_b200.score --gguf model.gguf --ids 1,15043,29892
+    python -m auratensor_b200.score --projections bf16                # prompts on the tensor cores
 
 ``BlockLlama`` is the model's forward pass (inference/LlamaModel.java:141-308)
 put together from the library's operators, for any number of sequences at once:
