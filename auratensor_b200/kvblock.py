@@ -58,10 +58,9 @@ class TokenBatch:
             _bad("slots and offsets must be int32, starts int64")
         if starts.numel() != n or offsets.numel() != n + 1:
             _bad(f"{n} slots need {n} starts and {n + 1} offsets, got {starts.numel()} and {offsets.numel()}")
-        if not (slots.is_cuda and starts.is_cuda and offsets.is_cuda):
-            _bad("batch tensors must be on a CUDA device")
-        if not slots.get_device() == starts.get_device() == offsets.get_device():
-            _bad("batch tensors must be on one device")
+        device = slots.get_device()  # -1: the host
+        if device < 0 or starts.get_device() != device or offsets.get_device() != device:
+            _bad("batch tensors must be on one device, a CUDA device")
         if not (slots.is_contiguous() and starts.is_contiguous() and offsets.is_contiguous()):
             _bad("batch tensors must be contiguous")
         if not (0 <= nTokens <= INT32_MAX and 0 <= maxTokens <= INT32_MAX and 0 <= maxEnd <= INT64_MAX):
